@@ -179,8 +179,9 @@ def prepare(case, seed):
     s.tok_seq = ints([i for i, n in enumerate(news) for _ in range(n)])
     s.tok_pos = ints([p + t for p, n in zip(pos0, news) for t in range(n)])
     s.view = SimpleNamespace(k=s.k, v=s.v, page_table=table.cuda(), page_size=ps, max_pages=max_pages)
-    # who shares what: a group's length, the sequence whose page table leads to it, its members' tokens
-    groups = [[i for i, q in enumerate(seqs) if q[0] == g] for g in range(case["groups"])]
+    # who shares what: a group's length, the sequence whose page table leads to it, its members' tokens (a sequence that shares
+    # nothing is a group of its own, of length 0)
+    groups = [[i for i, q in enumerate(seqs) if q[0] == g] for g in range(case["groups"])] + [[i] for i, q in enumerate(seqs) if q[0] < 0]
     toks = [[t for i in of for t in range(starts[i], starts[i + 1])] for of in groups]
     firsts = [0]
     for t in toks:
