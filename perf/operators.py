@@ -186,7 +186,7 @@ def prepare(case, seed):
     firsts = [0]
     for t in toks:
         firsts.append(firsts[-1] + len(t))
-    s.prefix = SimpleNamespace(n_groups=len(groups), most_tokens=max(len(t) for t in toks), most_len=max(seqs[of[0]][1] for of in groups),
+    s.prefix = SimpleNamespace(n_groups=len(groups), most_tokens=max(len(t) for t in toks), most_len=max(seqs[of[0]][1] for of in groups), most_own=max(q[2] + q[3] for q in seqs),
                                group_len=ints([seqs[of[0]][1] for of in groups]), group_seq=ints([of[-1] for of in groups]),
                                tok_first=ints(firsts), toks=ints([t for g in toks for t in g]), seq_skip=ints([q[1] for q in seqs]))
     H, K, D = case["heads"], case["kv_heads"], case["dim"]
