@@ -9,7 +9,8 @@ token that serves as both), a free list of pages and one page
 table `[slots, max_pages]`.  A sequence holds a slot, and in every group the
 pages that cover its length; groups with a window (or chunks) give pages back once
 no later token sees a key in them (those of the first `keep_first` tokens stay).  Slots and pages go back to the free lists
-when a sequence ends and are handed out again.  Next to the pages lies
+when a sequence ends and are handed out again.  Sequences that fork from one another share the full pages of their common
+beginning: such a page has several holders and goes back when the last of them lets it go.  Next to the pages lies
 fixed-size per-sequence state `[slots, ...]` for sites that declare some; it
 is zeroed when a slot is taken.
 
@@ -80,6 +81,7 @@ class CacheGroup:
         self.table_host = np.zeros((n_slots, max_pages), dtype=np.int32)
         self.kept_pages = -(-need.keep_first // page_size)  # pages at a sequence's start that never leave the window
         self.seq_pages: dict[int, dict[int, int]] = {}      # slot -> {page index in sequence: page}
+        self.holders: dict[int, int] = {}                   # pages that several sequences hold -> how many
         self.dirty: set[int] = set()
         shape = (len(sites), n_pages, page_size, need.n_kv_heads, need.head_dim)
         v_shape = shape[:3] + (need.n_v_heads or need.n_kv_heads, need.v_dim or need.head_dim)
@@ -110,6 +112,29 @@ class CacheGroup:
         if missing:
             self.dirty.add(slot)
 
+    def drop(self, page: int) -> None:
+        """One holder lets the page go; the last one frees it."""
+        n = self.holders.get(page, 1)
+        if n == 1:
+            self.pages.release(page)
+        elif n == 2:
+            del self.holders[page]
+        else:
+            self.holders[page] = n - 1
+
+    def place(self, slot: int, index: int, page: int) -> None:
+        """Page `index` of the sequence in `slot` is `page` from now on."""
+        self.seq_pages.setdefault(slot, {})[index] = page
+        self.table_host[slot, index] = page
+        self.dirty.add(slot)
+
+    def copy(self, src: list[int], dst: list[int], rows: Optional[list[int]] = None) -> None:
+        """Copy pages (their first `rows` rows) at every site, keys and values."""
+        if self.k is not None and src:
+            from .. import ops
+            with torch.cuda.device(self.k.device):
+                ops.copy_pages([self.k] if self.v is None else [self.k, self.v], src, dst, rows)
+
     def trim(self, slot: int, length: int) -> None:
         """Give back pages whose keys no later token sees: they have left the window or lie in an earlier chunk (the
         first tokens that the need keeps stay)."""
@@ -118,11 +143,11 @@ class CacheGroup:
         have = self.seq_pages.get(slot, {})
         first_live = self.need.first_key(length) // self.page_size
         for p in [p for p in have if self.kept_pages <= p < first_live]:
-            self.pages.release(have.pop(p))
+            self.drop(have.pop(p))
 
     def release(self, slot: int) -> None:
         for page in self.seq_pages.pop(slot, {}).values():
-            self.pages.release(page)
+            self.drop(page)
         self.dirty.discard(slot)
 
     def sync_tables(self) -> None:
@@ -161,6 +186,8 @@ class SequenceCache:
         self.max_pages = -(-max_context // page_size)
         self.slots = FreeList(max_slots, "sequence slot")
         self.lengths: dict[int, int] = {}
+        self.shares: dict[int, tuple[int, int]] = {}        # slot -> (number of its fork, tokens that the fork's sequences share)
+        self._forks = 0
         self.groups: list[CacheGroup] = []
         self.site_group: dict[int, tuple[int, int]] = {}
         by_need: dict[KVNeed, list[int]] = {}
@@ -201,7 +228,106 @@ class SequenceCache:
         self.slots.release(slot)
         for g in self.groups:
             g.release(slot)
+        self.shares.pop(slot, None)
         del self.lengths[slot]
+
+    def _fork_refusal(self, slot: int, n: int, length: Optional[int]) -> Optional[Exception]:
+        if slot not in self.lengths:
+            return ValueError(f"slot {slot} is not held by a sequence")
+        old = self.lengths[slot]
+        length = old if length is None else length
+        if n < 1:
+            return ValueError(f"a sequence forks into one further one at least, not {n}")
+        if not 0 <= length <= old:
+            return ValueError(f"a sequence of {old} tokens cannot fork at {length}")
+        if length != old and self.state_bytes:
+            return ValueError("a cache with fixed-size per-sequence state forks at a sequence's end only")
+        if n > self.slots.free_count:
+            return CacheFull(f"{n} more sequence slots are wanted, {self.slots.free_count} of {self.slots.n} are free")
+        for g in self.groups:
+            have, last = g.seq_pages.get(slot, {}), (length - 1) // self.page_size if length else -1
+            if g.need.bounded and any(p not in have for p in range(g.need.first_key(length) // self.page_size, last + 1)):
+                return ValueError("a windowed group has already released pages of the shared part")
+            want = n if length % self.page_size and last in have else 0
+            if want > g.pages.free_count:
+                return CacheFull(f"{want} more cache pages of {self.page_size} tokens are wanted, {g.pages.free_count} of "
+                                 f"{g.n_pages} are free")
+        return None
+
+    def can_fork(self, slot: int, n: int = 1, length: Optional[int] = None) -> Optional[str]:
+        """None if the sequence in `slot` can fork into `n` further ones, else the reason."""
+        why = self._fork_refusal(slot, n, length)
+        return None if why is None else str(why)
+
+    def fork(self, slot: int, n: int = 1, length: Optional[int] = None) -> list[int]:
+        """`n` new sequences that begin with the first `length` tokens (default: all) of the one in `slot`; returns their slots.
+        Full pages are shared; a last, partly filled page and fixed-size state are copied, so that every sequence goes on by
+        itself.  All or nothing.  The sequence and its new ones share their first `length` tokens from then on
+        (`shared_prefixes`); its last fork is the one that counts."""
+        why = self._fork_refusal(slot, n, length)
+        if why is not None:
+            raise why
+        length = self.lengths[slot] if length is None else length
+        new = [self.slots.acquire() for _ in range(n)]
+        full, rows = divmod(length, self.page_size)
+        for g in self.groups:
+            have = g.seq_pages.get(slot, {})
+            first = g.need.first_key(length) // self.page_size if g.need.bounded else 0
+            for p, page in have.items():
+                if p < full and (p >= first or p < g.kept_pages):
+                    g.holders[page] = g.holders.get(page, 1) + n
+                    for s in new:
+                        g.place(s, p, page)
+            if rows and full in have:
+                copies = g.pages.acquire_many(n)
+                for s, page in zip(new, copies):
+                    g.place(s, full, page)
+                g.copy([have[full]] * n, copies, [rows] * n)
+            g.sync_tables()
+        if self.states:
+            from .. import ops
+            with torch.cuda.device(self.device):
+                ops.copy_slots(list(self.states.values()), [slot] * n, new)
+        for s in new:
+            self.lengths[s] = length
+        if length:
+            if self.shares.get(slot, (0, 0))[1] != length:
+                self._forks += 1
+                self.shares[slot] = (self._forks, length)
+            for s in new:
+                self.shares[s] = self.shares[slot]
+        return new
+
+    def shared_prefixes(self, slots) -> list[tuple[int, list[int]]]:
+        """(tokens shared, numbers in `slots` of the sequences that share them) of the forks among these sequences, in the order
+        of the forks; one that is alone of its fork is listed too."""
+        found: dict[int, tuple[int, list[int]]] = {}
+        for i, slot in enumerate(slots):
+            share = self.shares.get(slot)
+            if share is not None:
+                found.setdefault(share[0], (share[1], []))[1].append(i)
+        return [found[f] for f in sorted(found)]
+
+    def compact(self) -> int:
+        """Move held pages from the rear of each group's pool to free ones at its front, so that the held pages are the pool's
+        first; returns how many were moved.  Tables follow; what is shared stays shared."""
+        moved = 0
+        for g in self.groups:
+            held = g.pages.held
+            front, rear = g.pages.vacant_below(len(held)), sorted(p for p in held if p >= len(held))
+            if not rear:
+                continue
+            g.copy(rear, front)
+            to = dict(zip(rear, front))
+            g.pages.swap(rear, front)
+            g.holders = {to.get(p, p): n for p, n in g.holders.items()}
+            for slot, have in g.seq_pages.items():
+                for index, page in have.items():
+                    if page in to:
+                        g.place(slot, index, to[page])
+            g.sync_tables()
+            moved += len(rear)
+        return moved
 
     def length(self, slot: int) -> int:
         return self.lengths[slot]
@@ -275,10 +401,24 @@ class SequenceCache:
             have = g.seq_pages.get(slot, {})
             if g.need.bounded and any(p not in have for p in range(g.need.first_key(length) // self.page_size, last + 1)):
                 raise ValueError("a windowed group has already released pages of the kept part")
+        # a last page that others hold too is copied before this sequence writes behind its kept rows
+        rows = length % self.page_size
+        own = [g for g in self.groups if rows and g.seq_pages.get(slot, {}).get(last) in g.holders]
+        for g in own:
+            if g.pages.free_count + sum(1 for p, page in g.seq_pages[slot].items() if p > last and page not in g.holders) < 1:
+                raise CacheFull(f"a page for the kept rows of a shared one is wanted, none of {g.n_pages} is free")
         for g in self.groups:
             have = g.seq_pages.get(slot, {})
             for p in [p for p in have if p > last]:
-                g.pages.release(have.pop(p))
+                g.drop(have.pop(p))
+            if g in own:
+                (page,) = g.pages.acquire_many(1)
+                g.copy([have[last]], [page], [rows])
+                g.drop(have[last])
+                g.place(slot, last, page)
+                g.sync_tables()
+        if self.shares.get(slot, (0, 0))[1] > length:
+            del self.shares[slot]                   # it has less than its fork shares
         self.lengths[slot] = length
 
     def view(self, site: int, state_site: Optional[int] = None) -> KVView:
@@ -306,7 +446,7 @@ class SequenceCache:
                 g.k.index_fill_(1, idx, value)
                 if g.v is not None:
                     g.v.index_fill_(1, idx, value)
-            for slot, have in g.seq_pages.items():
+            for slot, have in g.seq_pages.items():          # (a page that several hold is full: nothing of it is unused)
                 length = self.lengths.get(slot, 0)
                 for p, page in have.items():
                     first = max(0, length - p * self.page_size)
@@ -322,6 +462,9 @@ class SequenceCache:
         for g in self.groups:
             g.pages.check()
             owned = [page for pages in g.seq_pages.values() for page in pages.values()]
-            assert len(owned) == len(set(owned)), "a page belongs to two sequences"
+            counts: dict[int, int] = {}
+            for page in owned:
+                counts[page] = counts.get(page, 0) + 1
+            assert {p: n for p, n in counts.items() if n > 1} == g.holders, "a page belongs to two sequences"
             assert set(owned) == set(g.pages.held), "held pages and owned pages differ"
             assert set(g.seq_pages) <= set(self.slots.held), "pages owned by a slot that is free"

@@ -42,6 +42,17 @@ class FreeList:
         self._held.remove(item)
         self._free.append(item)
 
+    def vacant_below(self, limit: int) -> list[int]:
+        """The free items below `limit`, lowest first."""
+        return sorted(i for i in self._free if i < limit)
+
+    def swap(self, held: list[int], vacant: list[int]) -> None:
+        """What is held as `held` is held as `vacant` from now on, item for item."""
+        if len(held) != len(vacant) or not set(held) <= self._held or not set(vacant) <= set(self._free):
+            raise ValueError(f"only held {self.what}s can change places with free ones")
+        self._held = (self._held - set(held)) | set(vacant)
+        self._free = sorted((set(self._free) - set(vacant)) | set(held), reverse=True)
+
     def check(self) -> None:
         """Every item is free or held, exactly once."""
         assert len(self._free) == len(set(self._free)), f"a {self.what} is on the free list twice"

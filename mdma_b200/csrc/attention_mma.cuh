@@ -21,6 +21,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "mma_tiles.cuh"
 #include "ptx.cuh"
 
 namespace mdma {
@@ -28,33 +29,6 @@ namespace mdma {
 constexpr int kRows = 64;        // query rows per block (4 warps x 16)
 constexpr int kKeys = 64;        // keys per block of the stream
 constexpr int kAttnThreads = 128;
-
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
-    const int bytes = valid ? 16 : 0;       // 0: the 16 bytes are zero-filled
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
-}
-__device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                          uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-}
 
 struct AttnParams {
     const __nv_bfloat16* q; int q_stride;          // rows of the fused projection; queries first
@@ -92,12 +66,6 @@ template <bool EXT>
 __device__ __forceinline__ float score_log2(float raw, const AttnParams& p) {
     if (EXT && p.cap_log2 > 0.f) return fmaf(-2.0f * p.cap_log2, __fdividef(1.0f, 1.0f + exp2f(raw * p.cap_rate)), p.cap_log2);
     return raw * p.scale_log2;
-}
-
-// Tile shared-memory rows are DMAX elements wide; 16-byte chunk c of row r sits at chunk c ^ (r & 7).
-template <int DMAX>
-__device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
-    return (uint32_t)(row * DMAX * 2 + ((chunk ^ (row & 7)) << 4));
 }
 
 template <int DMAX, bool EXT = false>

@@ -1,0 +1,133 @@
+// Attention of a step whose sequences share prefixes: what the kernels of it have in common.
+//
+// Every sequence belongs to one group; a group's first `group_len` tokens lie in pages that its members' page tables share
+// (the rows of a partly filled last page are the same in each member's copy), so one member's table row leads to them all.
+// A query of a member sees the whole prefix and the keys [group_len, its position] of its own sequence.  With m the maximum
+// of the scores and l the sum of their exponentials over a set of keys, o the weighted sum of the values, two disjoint sets A, B join as
+//     m = max(mA, mB),  l = lA 2^(mA - m) + lB 2^(mB - m),  o = oA 2^(mA - m) + oB 2^(mB - m)
+// (scores in powers of two).  So a prefix is read once for the query rows of all members, which fill the rows of one tile,
+// every sequence's own keys are read by its own rows, and a last step joins the parts in a fixed order.
+#pragma once
+#include "common.cuh"
+
+namespace mdma {
+
+struct PrefixParams {
+    const void* q; long q_stride;                    // rows of the projection; queries first
+    const void* k_cache; const void* v_cache;        // [pages, page_size, kv_heads, head_dim]
+    const int* seq_start; const int* seq_pos0; const int* seq_slot; const int* tok_seq;
+    const int* page_table; int max_pages; int page_size; int n_pages;
+    const int* group_len; const int* group_seq; const int* tok_first; const int* toks; const int* seq_skip;
+    void* out;
+    float* part_o; float* part_ml;                   // [token][head][slot][head_dim], [token][head][slot][2]
+    int n_groups, n_seqs, n_tokens, max_new;
+    int n_heads, n_kv_heads, head_dim, group;
+    int pieces, own_splits;                          // a prefix in `pieces` pieces at most, own keys in `own_splits`: slots of the parts
+    float scale_log2;                                // scale * log2(e)
+    const float* sinks; float sink_rate;             // sinks[head] * sink_rate is in powers of two; null: none
+    int* status;
+};
+
+// Keys of a piece of a prefix of `len` tokens: a multiple of 128 that follows from the prefix alone, so that a sequence's sums
+// are cut at the same places whoever shares the step.
+__host__ __device__ __forceinline__ int prefix_piece(int len, int pieces) {
+    return ((len + pieces - 1) / pieces + 127) / 128 * 128;
+}
+__host__ __device__ __forceinline__ int prefix_pieces_used(int len, int pieces) {
+    if (len <= 0) return 0;
+    const int keys = prefix_piece(len, pieces);
+    return (len + keys - 1) / keys;
+}
+
+// Tile t of the prefixes' query rows, `tile_tokens` tokens each: which group, which of its tokens.  Groups without a prefix
+// have no tiles.  False: there is no such tile.
+struct PrefixTile { int g, first, count; };          // toks[first .. first + count)
+__device__ __forceinline__ bool prefix_tile(const PrefixParams& p, int t, int tile_tokens, PrefixTile& out) {
+    for (int g = 0; g < p.n_groups; ++g) {
+        if (p.group_len[g] <= 0) continue;
+        const int a = p.tok_first[g], n = p.tok_first[g + 1] - a, tiles = (n + tile_tokens - 1) / tile_tokens;
+        if (t < tiles) {
+            out.g = g; out.first = a + t * tile_tokens; out.count = min(tile_tokens, n - t * tile_tokens);
+            return true;
+        }
+        t -= tiles;
+    }
+    return false;
+}
+// The most tiles a step can have: every group leaves one partly filled.
+static inline long prefix_tiles_bound(const PrefixParams& p, int tile_tokens) {
+    return (long)p.n_tokens / tile_tokens + p.n_groups;
+}
+
+// out[token, head] from its parts: those of its prefix in order, then those of its own keys.  One warp a row.
+template <typename T>
+__global__ void __launch_bounds__(128)
+prefix_merge_kernel(const PrefixParams p) {
+    chain_release();
+    chain_wait();
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);         // token * heads + head
+    const int lane = threadIdx.x & 31;
+    if (row >= (long)p.n_tokens * p.n_heads) return;
+    const int slots = p.pieces + p.own_splits, D = p.head_dim;
+    const int used = prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces);
+    const float* ml = p.part_ml + row * slots * 2;
+    float m = -INFINITY;
+    for (int s = 0; s < used + p.own_splits; ++s) m = fmaxf(m, ml[2 * (s < used ? s : p.pieces + s - used)]);
+    const float sink = p.sinks ? p.sinks[row % p.n_heads] * p.sink_rate : -INFINITY;
+    float l = 0.f;
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int s = 0; s < used + p.own_splits; ++s) {
+        const int slot = s < used ? s : p.pieces + s - used;
+        const float ms = ml[2 * slot];
+        if (ms == -INFINITY) continue;
+        const float f = exp2f(ms - m);
+        l += f * ml[2 * slot + 1];
+        const float* o = p.part_o + (row * slots + slot) * D;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (lane + 32 * j < D) acc[j] = fmaf(f, o[lane + 32 * j], acc[j]);
+    }
+    if (p.sinks) l += exp2f(sink - m);
+    T* to = reinterpret_cast<T*>(p.out) + row * D;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (lane + 32 * j < D) to[lane + 32 * j] = from_float<T>(acc[j] / l);
+}
+
+// The arguments as one array of 64-bit words, in the order below (a step makes this call once a layer: converting thirty
+// arguments one by one costs the host more than the launches).
+static inline int prefix_params(const long long* w, int n_words, float scale, PrefixParams* out) {
+    MDMA_REQUIRE(n_words == 32, "prefix_attention: %d argument words", n_words);
+    PrefixParams& p = *out;
+    int i = 0;
+    auto ptr = [&]() { return (void*)(uintptr_t)w[i++]; };
+    auto num = [&]() { return (int)w[i++]; };
+    p.q = ptr(); p.q_stride = (long)w[i++];
+    p.k_cache = ptr(); p.v_cache = ptr();
+    p.seq_start = (const int*)ptr(); p.seq_pos0 = (const int*)ptr(); p.seq_slot = (const int*)ptr(); p.tok_seq = (const int*)ptr();
+    p.page_table = (const int*)ptr(); p.max_pages = num(); p.page_size = num(); p.n_pages = num();
+    p.group_len = (const int*)ptr(); p.group_seq = (const int*)ptr(); p.tok_first = (const int*)ptr(); p.toks = (const int*)ptr();
+    p.seq_skip = (const int*)ptr();
+    p.out = ptr();
+    float* scratch = (float*)ptr();
+    const long long floats = w[i++];
+    p.n_groups = num(); p.n_seqs = num(); p.n_tokens = num(); p.max_new = num();
+    p.n_heads = num(); p.n_kv_heads = num(); p.head_dim = num();
+    p.pieces = num(); p.own_splits = num();
+    p.sinks = (const float*)ptr();
+    p.status = (int*)ptr();
+    p.sink_rate = w[i++] ? 1.0f : 1.4426950408889634f;      // the sinks come times log2(e), or as they are
+    p.scale_log2 = scale * 1.4426950408889634f;
+    MDMA_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0, "prefix_attention: %d heads over %d kv heads", p.n_heads, p.n_kv_heads);
+    MDMA_REQUIRE(p.head_dim > 0 && p.head_dim <= 256, "prefix_attention: head_dim %d is beyond the limit of 256", p.head_dim);
+    MDMA_REQUIRE(p.page_table && p.page_size > 0 && p.max_pages > 0, "prefix_attention: bad cache geometry");
+    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 1 && p.own_splits >= 1, "prefix_attention: bad sizes");
+    MDMA_REQUIRE(scale > 0.f, "prefix_attention: the score scale must be positive");
+    p.group = p.n_heads / p.n_kv_heads;
+    const long long slots = (long long)p.n_tokens * p.n_heads * (p.pieces + p.own_splits), need = slots * (p.head_dim + 2);
+    MDMA_REQUIRE(scratch && floats >= need, "prefix_attention: %lld floats of scratch are needed, %lld given", need, floats);
+    p.part_o = scratch; p.part_ml = scratch + slots * p.head_dim;
+    return 0;
+}
+
+}  // namespace mdma

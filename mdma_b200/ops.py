@@ -1110,3 +1110,121 @@ def matrix_memory_token(proj, cols, g_col: int, i_bias, f_bias, cap: float, q_sc
           ctypes.c_long(split_stride), _i(proj.shape[1]), _i(q_col), _i(k_col), _i(v_col), _i(g_col), _i(i_col), _i(f_col),
           _ptr(i_bias), _ptr(f_bias), _i(_same_dtype(i_bias, f_bias)), _f(cap), _f(q_scale), _ptr(norm_w), _i(dtype_code(norm_w.dtype)),
           _ptr(ctx.seq_slot), sp, ss, _ptr(out), _i(ctx.n_seqs), _i(heads), _i(dim), _i(vdim), _f(eps), _f(out_scale), _stream())
+
+
+# ---- pages of the cache, and attention of sequences that share their beginning ------------------------------------------------
+def _need_current(t: torch.Tensor) -> None:
+    """A launch goes to a stream of the current device: tensors of another one are refused."""
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def copy_pages(pools, src, dst, rows=None) -> None:
+    """Page dst[i] of every pool becomes a copy of page src[i], at every site; with `rows` only its first rows[i] rows do.
+    `pools`: contiguous tensors [sites, pages, page_size, ...] with as many pages and rows a page (keys and values of a cache
+    group; heads, sizes and dtypes may differ).  `src`, `dst`, `rows`: numbers on the host; they travel with the launch, so
+    nothing is uploaded and a captured launch keeps them.  A page may be copied to several others, but is not written twice
+    and not both read and written in one call."""
+    pools = list(pools)
+    if not pools:
+        return
+    _need_cuda(*pools)
+    n_pages, page_size = pools[0].shape[1:3]
+    words = []
+    for p in pools:
+        if p.device != pools[0].device or p.dim() < 3 or p.shape[1:3] != (n_pages, page_size) or not p.is_contiguous():
+            raise KernelError("copy_pages takes contiguous pools [sites, pages, page_size, ...] of one device with the same "
+                              "pages and page size")
+        size = p.element_size()
+        words += (p.data_ptr(), p.stride(1) * size, p.stride(0) * size, p.stride(2) * size, p.shape[0])
+    _need_current(pools[0])
+    n = len(src)
+    if len(dst) != n or (rows is not None and len(rows) != n):
+        raise KernelError(f"copy_pages: {n} pages to copy from, {len(dst)} to copy to, {n if rows is None else len(rows)} row counts")
+    if n == 0 or pools[0].numel() == 0:
+        return
+    ints = ctypes.c_int * n
+    launches = ctypes.c_int(0)
+    _call("core", "mdma_copy_pages", (ctypes.c_longlong * len(words))(*words), _i(len(pools)), _i(n_pages), _i(page_size),
+          ints(*src), ints(*dst), None if rows is None else ints(*rows), _i(n), ctypes.byref(launches), _stream(), launches=0)
+    global LAUNCHES
+    LAUNCHES += launches.value
+
+
+def copy_slots(states, src, dst) -> None:
+    """Row dst[i] of every per-sequence state [slots, ...] becomes a copy of row src[i]."""
+    copy_pages([s.view(1, s.shape[0], 1, -1) for s in states], src, dst)
+
+
+def prefix_split(tile_rows: int, blocks_wanted: int, tokens: int, seqs: int, max_new: int, most_len: int, most_own: int, n_heads: int,
+                 n_kv_heads: int) -> tuple[int, int]:
+    """(pieces of a prefix, pieces of a sequence's own keys) for blocks of `tile_rows` query rows of one kv head, so that about
+    `blocks_wanted` blocks share the work."""
+    group = n_heads // n_kv_heads
+    tile_tokens = max(1, tile_rows // group)
+    tiles = -(-tokens // tile_tokens) * n_kv_heads * max(1, -(-group // tile_rows))
+    pieces = max(1, min(blocks_wanted // tiles, 32, -(-most_len // 128)))
+    own = -(-max_new // tile_tokens) * seqs * n_kv_heads * max(1, -(-group // tile_rows))
+    return pieces, max(1, min(blocks_wanted // own, 32, -(-most_own // 128)))
+
+
+def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, pieces: int, own_splits: int, scratch, sinks, status,
+                 sinks_log2: bool):
+    """The arguments of the prefix attention kernels as one array (see csrc/prefix.cuh)."""
+    g = ctx.prefix
+    words = (q.data_ptr(), q.stride(0), view.k.data_ptr(), view.v.data_ptr(), ctx.seq_start.data_ptr(), ctx.seq_pos0.data_ptr(),
+             ctx.seq_slot.data_ptr(), ctx.tok_seq.data_ptr(), view.page_table.data_ptr(), view.max_pages, view.page_size,
+             view.k.shape[0], g.group_len.data_ptr(), g.group_seq.data_ptr(), g.tok_first.data_ptr(), g.toks.data_ptr(),
+             g.seq_skip.data_ptr(), out.data_ptr(), scratch.data_ptr(), scratch.numel(), g.n_groups, ctx.n_seqs, ctx.n_tokens,
+             ctx.max_new, n_heads, n_kv_heads, head_dim, pieces, own_splits, 0 if sinks is None else sinks.data_ptr(),
+             0 if status is None else status.data_ptr(), int(sinks_log2))
+    return (ctypes.c_longlong * 32)(*words)
+
+
+def prefix_checks(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, sinks) -> None:
+    """What the prefix attention kernels cannot check of their arguments."""
+    g = ctx.prefix
+    ints = (ctx.seq_start, ctx.seq_pos0, ctx.seq_slot, ctx.tok_seq, view.page_table, g.group_len, g.group_seq, g.tok_first, g.toks,
+            g.seq_skip)
+    _need_cuda(q, view.k, view.v, out, sinks, *ints)
+    _need_current(q)
+    if any(t.dtype != torch.int32 for t in ints):
+        raise KernelError("positions, page tables and groups are int32")
+    if (view.k.dtype != q.dtype or view.v.dtype != q.dtype or out.dtype != q.dtype or q.dim() != 2 or q.stride(1) != 1
+            or not view.k.is_contiguous() or not view.v.is_contiguous() or not out.is_contiguous() or not view.page_table.is_contiguous()):
+        raise KernelError("queries, caches and results have one dtype; caches and results are contiguous")
+    if (n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads or view.k.shape != view.v.shape
+            or tuple(view.k.shape[1:]) != (view.page_size, n_kv_heads, head_dim) or q.shape[0] < ctx.n_tokens
+            or q.shape[1] < n_heads * head_dim or out.shape[0] < ctx.n_tokens or out.shape[1] != n_heads * head_dim):
+        raise KernelError(f"{n_heads} heads over {n_kv_heads} kv heads of {head_dim} do not fit queries {tuple(q.shape)}, caches "
+                          f"{tuple(view.k.shape)} and results {tuple(out.shape)}")
+    if (g.group_len.numel() < g.n_groups or g.group_seq.numel() < g.n_groups or g.tok_first.numel() < g.n_groups + 1
+            or g.toks.numel() < ctx.n_tokens or g.seq_skip.numel() < ctx.n_seqs):
+        raise KernelError("the groups' tables are shorter than the step")
+    if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != n_heads):
+        raise KernelError("sinks are one float a head")
+
+
+def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
+                     sinks: Optional[torch.Tensor] = None, scratch: Optional[torch.Tensor] = None) -> None:
+    """Causal grouped-query attention of a step whose sequences share prefixes, on the CUDA cores (float32, or bfloat16 with
+    float arithmetic; head sizes up to 256).  `ctx.prefix` says who shares what (`cache.PrefixGroups`): every key of a shared
+    prefix is read once for the queries of all the group's members, every sequence's own keys by its own queries, and the two
+    parts of each softmax are joined.  The prefix must be in the cache before the step (its length is at most every
+    member's `seq_pos0`).  `sinks` [n_heads] floats join their heads' denominators once.  `scratch`: floats for the parts
+    (without it they are allocated for the call)."""
+    prefix_checks(ctx, q, view, out, n_heads, n_kv_heads, head_dim, sinks)
+    if ctx.n_tokens == 0:
+        return
+    g = ctx.prefix
+    seqs = getattr(ctx, "most_seqs", None) or ctx.n_seqs
+    tokens = seqs if ctx.max_new == 1 else ctx.n_tokens
+    pieces, own = prefix_split(32, 4 * 148, tokens, seqs if ctx.max_new == 1 else ctx.n_seqs, ctx.max_new, g.most_len, g.most_own,
+                               n_heads, n_kv_heads)
+    need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2)
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+    elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need:
+        raise KernelError(f"prefix attention needs {need} floats of scratch, {scratch.numel()} given")
+    words = prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sinks, None, False)
+    _call("core", "mdma_prefix_attention_simple", words, _i(32), _f(scale), _i(dtype_code(q.dtype)), _stream(), launches=2)

@@ -602,6 +602,7 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
     assert view.k.shape[-2:] == (n_kv_heads * maps, dim) and view.v.shape[-2:] == (n_kv_heads, v_dim)
     for t in (sink_log2, slope_log2):
         assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n_heads)
+    own_st = st
     st = st or _device_state(q.device)
     flush_pending(q.device, st)
     group = n_heads // n_kv_heads
@@ -634,3 +635,33 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
         return None
     sums = ctx.n_tokens * n_heads * maps * splits * v_dim
     return st.scratch[:sums], st.scratch[sums:need], splits
+
+
+# ---- attention of sequences that share their beginning (csrc/attention_prefix.cu) ------------------------------------------
+def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
+                     sink_log2: Optional[torch.Tensor] = None, st: Optional[TensorState] = None) -> None:
+    """`ops.prefix_attention` in bfloat16 on the tensor cores (the geometries of `attention_supported`).  `sink_log2`: the sinks
+    times log2(e).  `st`: the engine's state, whose scratch takes the parts (without it they are allocated for the call)."""
+    if q.dtype != torch.bfloat16:
+        raise KernelError("the tensor-core attention takes bfloat16")
+    if not attention_supported(n_heads, n_kv_heads, head_dim):
+        raise KernelError(f"the tensor-core attention does not take {n_heads} heads over {n_kv_heads} kv heads of {head_dim}")
+    ops.prefix_checks(ctx, q, view, out, n_heads, n_kv_heads, head_dim, sink_log2)
+    if ctx.n_tokens == 0:
+        return
+    own_st = st
+    st = st or _device_state(q.device)
+    flush_pending(q.device, st)
+    g = ctx.prefix
+    seqs = getattr(ctx, "most_seqs", None) or ctx.n_seqs
+    one = ctx.max_new == 1
+    pieces, own = ops.prefix_split(64, 2 * st.sms, seqs if one else ctx.n_tokens, seqs if one else ctx.n_seqs, ctx.max_new, g.most_len,
+                                   g.most_own, n_heads, n_kv_heads)
+    need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2)
+    if own_st is not None:
+        st.need(need, "attention over shared prefixes")
+        scratch = st.scratch
+    else:
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+    words = ops.prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sink_log2, st.status, True)
+    _call("tensor", "mdma_prefix_attention", words, _i(32), _f(scale), _stream(), launches=2)
