@@ -42,6 +42,9 @@ def cmd_run(args) -> int:
     if args.max_tokens <= 0:
         print("--max-tokens must be positive", file=sys.stderr)
         return 2
+    if args.n <= 0:
+        print("--n must be positive", file=sys.stderr)
+        return 2
     need_ctx = max(len(p) for p in prompts) + args.max_tokens
     source = {"model_dir": args.model}
     if args.random_weights is not None:
@@ -50,7 +53,7 @@ def cmd_run(args) -> int:
         with open(path, "r", encoding="utf-8") as f:
             source = {"config": json.load(f), "seed": args.random_weights}
     try:
-        engine = Engine(**source, dtype=args.dtype, max_batch=min(args.max_batch, len(prompts)),
+        engine = Engine(**source, dtype=args.dtype, max_batch=min(args.max_batch, len(prompts) * args.n),
                         max_context=args.max_context or None, reserve_mib=args.reserve_mib,
                         vram_bytes=args.vram_bytes, context_hint=need_ctx,
                         history_cap=max(64, args.repetition_window))
@@ -63,7 +66,7 @@ def cmd_run(args) -> int:
         params = SamplingParams(args.temperature, args.top_p, args.min_p, args.repetition_penalty,
                                 args.repetition_window, args.seed)
     stop = parse_ids(args.stop_ids) if args.stop_ids else list(engine.spec.stop_token_ids)
-    outs = Generator(engine).generate(prompts, args.max_tokens, params, stop)
+    outs = Generator(engine).generate(prompts, args.max_tokens, params, stop, n=args.n)
     for o in outs:
         if args.json or os.environ.get("MDMA_JSON") is not None:
             print(json.dumps({"prompt_tokens": o.prompt_tokens, "tokens": o.tokens,
@@ -108,6 +111,7 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--prompt", dest="more_prompts", type=parse_ids, action="append",
                      help="a further prompt of the same batch (repeatable)")
     run.add_argument("--max-tokens", type=int, default=32)
+    run.add_argument("--n", type=int, default=1, help="completions of every prompt; the prompt is computed and kept once")
     run.add_argument("--json", action="store_true")
     run.add_argument("--greedy", action="store_true", help="argmax, no penalty (the default temperature is 0 as well)")
     run.add_argument("--temperature", type=float, default=0.0)

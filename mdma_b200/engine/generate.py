@@ -13,7 +13,8 @@ context ends with reason "context_limit".
 
 The loop decides; it does not compute.  It needs an object with `acquire()`,
 `release(slot)`, `step(entries) -> logits`, `max_context`, `max_slots`,
-`fits(list of (prompt length, budget))`, and a sampler with
+`fits(list of (prompt length, budget))`, for several completions of a
+prompt also `fork(slot, n)` and `fan_out(logits, counts)`, and a sampler with
 `sample(logits, params, requests, steps, histories) -> (tokens, flags)`.
 """
 from __future__ import annotations
@@ -44,7 +45,7 @@ class Output:
 
 @dataclass
 class _Live:
-    request: int
+    request: int                # number of the output
     slot: int
     budget: int
     context_limited: bool
@@ -78,7 +79,7 @@ class Generator:
         batches, cur = [], []
         for i, size in enumerate(sizes):
             trial = cur + [i]
-            if len(trial) <= self.engine.max_slots and self.engine.fits([sizes[j] for j in trial]):
+            if sum(sizes[j][2] if len(sizes[j]) > 2 else 1 for j in trial) <= self.engine.max_slots and self.engine.fits([sizes[j] for j in trial]):
                 cur = trial
                 continue
             if not cur:
@@ -97,18 +98,30 @@ class Generator:
                  params: Optional[SamplingParams] = None, stop_ids: Sequence[int] = (),
                  cancelled: Optional[Callable[[], bool]] = None,
                  on_token: Optional[Callable[[int, int], None]] = None,
-                 use_graphs: Optional[bool] = None) -> list[Output]:
+                 use_graphs: Optional[bool] = None, n: int = 1) -> list[Output]:
+        """`n`: completions of every prompt (outputs i * n .. i * n + n - 1 are prompt i's).  A prompt is computed once; its
+        sequence forks and its completions share what it holds.  (More completions than the engine has slots for take
+        several turns, the prompt computed in each.)"""
+        if n < 1:
+            raise ValueError("every prompt takes one completion at least")
         params = params or SamplingParams.greedy()
         params.validate()
         stop = frozenset(int(s) for s in stop_ids)
         if params.repetition_penalty != 1.0 and hasattr(self.sampler, "ensure_history"):
             self.sampler.ensure_history(params.repetition_window)       # refuses a window it has no room for
         budgets = [token_budget(len(p), max_tokens, self.engine.max_context) for p in prompts]
-        outputs = [Output(list(p)) for p in prompts]
-        sizes = [(len(p), b) for p, (b, _) in zip(prompts, budgets)]
+        outputs = [Output(list(p)) for p in prompts for _ in range(n)]
         graphs = self.use_graphs if use_graphs is None else use_graphs
+        # (prompt, its outputs): a prompt's completions start together, as many as can be live at once
+        turns = []
+        for i, p in enumerate(prompts):
+            most = 1
+            while most < n and most < self.engine.max_slots and self.engine.fits([(len(p), budgets[i][0], most + 1)]):
+                most += 1
+            turns += [(i, list(range(i * n + j, i * n + min(n, j + most)))) for j in range(0, n, most)]
+        sizes = [(len(prompts[i]), budgets[i][0]) + ((len(of),) if len(of) > 1 else ()) for i, of in turns]
         for batch in self.plan_batches(sizes):
-            self._run_batch(batch, prompts, budgets, outputs, params, stop, cancelled, on_token, graphs)
+            self._run_batch([turns[t] for t in batch], prompts, budgets, outputs, params, stop, cancelled, on_token, graphs)
         return outputs
 
     def _absorb(self, live, tokens, flags, outputs, stop, on_token) -> list:
@@ -138,7 +151,7 @@ class Generator:
         return survivors
 
     def _run_batch(self, batch, prompts, budgets, outputs, params, stop, cancelled, on_token, graphs) -> None:
-        live = [_Live(r, self.engine.acquire(), budgets[r][0], budgets[r][1]) for r in batch]
+        live = [_Live(of[0], self.engine.acquire(), *budgets[i]) for i, of in batch]
         penalised = params.repetition_penalty != 1.0 and params.repetition_window > 0
         session = None
         session_fresh = False          # whether the session's device buffers describe the live sequences
@@ -156,8 +169,19 @@ class Generator:
                 cancel_all()
                 return
             # all prompts of the batch in one step
-            entries = [StepEntry(s.slot, list(prompts[s.request]), [len(prompts[s.request]) - 1]) for s in live]
+            entries = [StepEntry(s.slot, list(prompts[i]), [len(prompts[i]) - 1]) for s, (i, _) in zip(live, batch)]
             logits = self.engine.step(entries)
+            if any(len(of) > 1 for _, of in batch):
+                first = live
+                live = list(first)              # (every slot that is held is in `live`, whatever happens)
+                forked = []
+                for s, (i, of) in zip(first, batch):
+                    more = [_Live(r, slot, *budgets[i]) for r, slot in
+                            zip(of[1:], self.engine.fork(s.slot, len(of) - 1) if len(of) > 1 else ())]
+                    live += more
+                    forked += [s] + more
+                live = forked
+                logits = self.engine.fan_out(logits, [len(of) for _, of in batch])
             tokens, flags = self.sampler.sample(logits, params, [s.request for s in live],
                                                 [s.steps for s in live], histories_of(live))
             if hasattr(self.engine, "check_status"):
@@ -205,12 +229,13 @@ def generate(model_dir: str, prompts: Sequence[Sequence[int]], max_tokens: int =
              temperature: float = 0.0, seed: int = 0, stop_ids: Optional[Sequence[int]] = None,
              dtype: str = "bfloat16", top_p: float = 1.0, min_p: float = 0.0,
              repetition_penalty: float = 1.0, repetition_window: int = 64,
-             max_batch: int = 8, max_context: Optional[int] = None, use_graphs: bool = True,
+             max_batch: int = 8, max_context: Optional[int] = None, use_graphs: bool = True, n: int = 1,
              **engine_args) -> list[Output]:
-    """One call from a model folder and token-id prompts to generated token ids."""
+    """One call from a model folder and token-id prompts to generated token ids; `n` completions of every prompt, which is
+    computed once and shared by them."""
     from .step import Engine
     engine = Engine(model_dir, dtype=dtype, max_batch=max_batch, max_context=max_context, **engine_args)
     params = SamplingParams(temperature, top_p, min_p, repetition_penalty, repetition_window, seed)
     if stop_ids is None:
         stop_ids = engine.spec.stop_token_ids
-    return Generator(engine, use_graphs=use_graphs).generate(prompts, max_tokens, params, stop_ids)
+    return Generator(engine, use_graphs=use_graphs).generate(prompts, max_tokens, params, stop_ids, n=n)

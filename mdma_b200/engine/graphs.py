@@ -44,6 +44,8 @@ class DecodeSession:
             b["ids"], b["tok_pos"], b["seq_slot"], b["seq_pos0"], b["arange"])
         self.ring, self.ring_counter = engine.token_ring, engine.ring_counter
         self.logits = engine.logits
+        self._prefix_words = b["prefix"]              # who shares what among the live sequences
+        self.prefix = None
         self._rows = b["rows"]                        # ids, tok_pos, seq_slot, seq_pos0: one upload
         self._host = torch.zeros(4, cap, dtype=torch.int32).pin_memory()
         self._host_np = self._host.numpy()            # the same pinned words, written without a tensor in between
@@ -84,6 +86,12 @@ class DecodeSession:
         h[0, :B], h[1, :B], h[2, :B], h[3, :B] = list(tokens), pos, self.slots, pos
         self._rows.copy_(self._host, non_blocking=True)
         self.engine.h2d_bytes += 4 * self._host.numel()
+        self.prefix = self.engine.prefix_groups(self.slots, pos, [1] * B)
+        if self.prefix is not None:
+            words = torch.from_numpy(self.prefix.words())
+            self._prefix_words[:words.numel()].copy_(words)
+            self.prefix.bind(self._prefix_words)
+            self.engine.h2d_bytes += 4 * words.numel()
 
     # ---- one step ----------------------------------------------------------
     @property
@@ -99,6 +107,9 @@ class DecodeSession:
         ctx.n_tokens = ctx.n_seqs = ctx.n_want = B
         ctx.max_new, ctx.max_len = 1, self._bucket
         ctx.decode_only = True
+        ctx.prefix = self.prefix
+        if self.prefix is not None:         # as `Engine.prefix_groups` bounds a step of its own
+            self.prefix.most_own = self._bucket - self.prefix.least_skip
         ctx.host_seq_new, ctx.host_seq_pos0, ctx.host_seq_slot = [1] * B, None, list(self.slots)
         return ctx
 
@@ -147,6 +158,8 @@ class DecodeSession:
         for _ in range(n):
             if use_graph and self.graph_safe:
                 key = (B, self._bucket, draws)
+                if self.prefix is not None:       # what the grids and the tables' places follow from
+                    key += (self.prefix.n_groups, self.prefix.most_len, self.prefix.least_skip)
                 g = self.graphs.get(key)
                 if g is None:
                     # The first step at this batch size runs eagerly (it loads kernels); the same

@@ -22,7 +22,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
-from ..cache import SequenceCache
+from ..cache import PrefixGroups, SequenceCache
 from ..config import load_config
 from ..parts.base import Runtime
 from ..weights import load_tensors, random_tensor, resident_dtype, stored_dtypes
@@ -62,6 +62,7 @@ class StepContext:
         self.max_new = self.max_len = 0
         self.most_seqs = None               # the most sequences the engine holds, and the longest context (kernels may
         self.most_len = None                # plan for them)
+        self.prefix = None                  # which sequences share their beginning (`cache.PrefixGroups`; None: none do)
         self.ids = self.tok_seq = self.tok_pos = self.seq_slot = self.seq_start = self.seq_pos0 = None
         self.want_rows = None
 
@@ -101,13 +102,15 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
         dt = torch.float32 if kind == "f32" else dtype
         lay.workspace[name] = carver.take("workspace", (chunk_tokens, cols), dt)
     lay.logits = carver.take("logits", (logit_rows, model.spec.vocab_size), torch.float32)
-    lay.meta_cap = 6 * chunk_tokens + 4 * max_slots + logit_rows + 16
+    # (ids, positions, .. of a pass, and who shares what)
+    lay.meta_cap = 6 * chunk_tokens + 4 * max_slots + logit_rows + 16 + chunk_tokens + 4 * max_slots + 1
     lay.meta_dev = carver.take("metadata", (lay.meta_cap,), torch.int32)
     # the replayed decode step reads its inputs from here: ids, positions (twice), slots, 0..cap
     # (the first four side by side: one copy brings them)
     rows = carver.take("metadata", (4, max_slots), torch.int32)
     lay.decode = {name: rows[i] if rows is not None else None for i, name in enumerate(("ids", "tok_pos", "seq_slot", "seq_pos0"))}
     lay.decode["rows"] = rows
+    lay.decode["prefix"] = carver.take("metadata", (5 * max_slots + 1,), torch.int32)
     lay.decode["arange"] = carver.take("metadata", (max_slots + 1,), torch.int32)
     lay.sampler = DeviceSampler(model.spec.vocab_size, max_slots, device, history_cap, alloc=carver.taker("sampler"))
     # the result words (tokens, flags, status) of the last `run_ahead` replayed decode steps
@@ -124,11 +127,30 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
     if dtype == torch.bfloat16:
         from .. import ops_tensor
         floats = ops_tensor.scratch_floats_bound(sms, chunk_tokens, max_slots, shapes)
+    floats = max(floats, prefix_floats(model, dtype, sms, max_slots, max_context))
     lay.scratch_floats = floats
     lay.tc_sk_flags = carver.take("kernel_scratch", (max(512, 4 * sms),), torch.int32)
     lay.tc_scratch = carver.take("kernel_scratch", (max(floats, 1),), torch.float32)
     lay.tables = carver.take("tables", (max(model.device_tensor_bytes(), 1),), torch.uint8)
     return lay
+
+
+def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_context: int) -> int:
+    """Scratch for single-token steps over shared prefixes: the parts of every sequence's softmaxes (steps of several tokens
+    use it as far as it goes)."""
+    from types import SimpleNamespace
+
+    from .. import ops, ops_tensor
+    ctx = SimpleNamespace(max_new=1, n_seqs=max_slots, n_tokens=max_slots, most_seqs=max_slots)
+    most = SimpleNamespace(most_len=max_context, most_own=max_context)
+    need = 0
+    for part in model.all_parts():
+        for heads, kv_heads, head_dim in getattr(part, "prefix_shapes", list)():
+            parts = sum(ops.prefix_plan(ctx, most, heads, kv_heads))
+            if dtype == torch.bfloat16 and ops_tensor.attention_supported(heads, kv_heads, head_dim):
+                parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, sms)))
+            need = max(need, max_slots * heads * parts * (head_dim + 2))
+    return need
 
 
 def _plan_dict(carver: Carver, cache: SequenceCache, page_size, max_slots, chunk_tokens, logit_rows) -> dict:
@@ -271,6 +293,7 @@ class Engine:
                 # the kernels' status word lies beside the sampler's tokens: one copy brings both to the host
                 self.rt.tc = ops_tensor.TensorState(self.device, lay.scratch_floats, sms=sms, status=self.sampler.extra,
                                                     sk_flags=lay.tc_sk_flags, scratch=lay.tc_scratch)
+            self.rt.prefix_scratch = lay.tc_scratch
             tables = Carver(lay.tables)
             self.rt.alloc = tables.taker("tables")
             self.model.bind(lay.tensors, self.rt)
@@ -332,7 +355,7 @@ class Engine:
 
     def generate(self, prompts, max_tokens: int = 32, temperature: float = 0.0, seed: int = 0,
                  stop_ids=None, top_p: float = 1.0, min_p: float = 0.0, repetition_penalty: float = 1.0,
-                 repetition_window: int = 64, use_graphs: bool = True):
+                 repetition_window: int = 64, use_graphs: bool = True, n: int = 1):
         """Generate from token-id prompts on this engine; see `mdma_b200.generate`."""
         from ..sampling.params import SamplingParams
         from .generate import Generator
@@ -340,7 +363,7 @@ class Engine:
             self._generator = Generator(self)
         params = SamplingParams(temperature, top_p, min_p, repetition_penalty, repetition_window, seed)
         stop = self.spec.stop_token_ids if stop_ids is None else stop_ids
-        return self._generator.generate(prompts, max_tokens, params, stop, use_graphs=use_graphs)
+        return self._generator.generate(prompts, max_tokens, params, stop, use_graphs=use_graphs, n=n)
 
     def decode_session(self):
         """The engine's `DecodeSession` (decode steps replayed as CUDA graphs).  There is one:
@@ -357,12 +380,56 @@ class Engine:
     def release(self, slot: int) -> None:
         self.cache.release(slot)
 
+    def fork(self, slot: int, n: int = 1, length: Optional[int] = None) -> list[int]:
+        """`n` new sequences that go on from the first `length` tokens (default: all) of the one in `slot`; returns their slots.
+        What they have in common is kept once, and later steps read it once for all of them (`SequenceCache.fork`)."""
+        return self.cache.fork(slot, n, length)
+
+    def compact(self) -> int:
+        """Bring the pages that are held to the front of the cache's pools; returns how many moved (`SequenceCache.compact`)."""
+        return self.cache.compact()
+
+    def fan_out(self, logits: torch.Tensor, counts: Sequence[int]) -> torch.Tensor:
+        """Row i of the last step's logits as often as counts[i] says, one copy behind the other, in the engine's own buffer."""
+        total = sum(counts)
+        if len(counts) != logits.shape[0] or min(counts, default=1) < 1 or total > self.logit_rows:
+            raise StepError(f"{logits.shape[0]} rows of logits cannot become {list(counts)} in {self.logit_rows}")
+        from .. import ops
+        at = total
+        for row in range(len(counts) - 1, -1, -1):        # from the last: no row is written over before it was copied
+            at -= counts[row]
+            to = [r for r in range(at, at + counts[row]) if r != row]
+            ops.copy_slots([self.logits], [row] * len(to), to)
+        return self.logits[:total]
+
     def fits(self, sizes) -> bool:
-        """Whether sequences of (prompt length, token budget) can be live together in an empty cache."""
-        if len(sizes) > self.max_slots:
-            return False
-        pages = sum(-(-(p + b - 1) // self.page_size) for p, b in sizes)
-        return pages <= self.cache.n_pages and all(p + b - 1 <= self.max_context for p, b in sizes)
+        """Whether sequences of (prompt length, token budget), or (prompt length, token budget, sequences that go on from that
+        prompt), can be live together in an empty cache."""
+        pages = slots = 0
+        for p, b, *n in sizes:
+            n = n[0] if n else 1
+            shared = p // self.page_size if n > 1 else 0
+            slots += n
+            # (before the prompt's sequence has let go of anything, every other one has a copy of its last page)
+            pages += shared + n * (-(-(p + b - 1) // self.page_size) - shared)
+            if p + b - 1 > self.max_context:
+                return False
+        return slots <= self.max_slots and pages <= self.cache.n_pages
+
+    def prefix_groups(self, slots: Sequence[int], pos0: Sequence[int], new: Sequence[int]):
+        """Who shares what in a step of these sequences, or None where nobody does.  Of single tokens the bounds are rounded to
+        multiples of 1,024 as the replayed graphs see them (a graph serves every batch within its bounds), so that a step on
+        its own adds up in the same order."""
+        shared = [(length, members) for length, members in self.cache.shared_prefixes(slots)
+                  if all(pos0[m] >= length for m in members)]
+        if not shared:
+            return None
+        groups = PrefixGroups(shared, pos0, new)
+        if max(new) == 1:
+            up = lambda n: min(self.max_context, -(-n // 1024) * 1024)  # noqa: E731
+            groups.most_len, groups.least_skip = up(groups.most_len), groups.least_skip // 1024 * 1024
+            groups.most_own = up(max(pos0) + 1) - groups.least_skip
+        return groups
 
     # ---- the step ----------------------------------------------------------
     def _validate(self, entries: Sequence[StepEntry]) -> None:
@@ -468,7 +535,10 @@ class Engine:
         want_rows = [row for _, row in wanted]
         ids, tok_seq, tok_pos = np.concatenate(ids), np.concatenate(tok_seq), np.concatenate(tok_pos)
         T, B, W = len(ids), len(pieces), len(want_rows)
+        groups = self.prefix_groups(seq_slot, seq_pos0, [take for _, _, take in pieces])
         fields = [ids, tok_seq, tok_pos, seq_slot, seq_start, seq_pos0, want_rows]
+        if groups is not None:
+            fields.append(groups.words())
         flat = np.concatenate([np.asarray(f, dtype=np.int32) for f in fields])
         n = flat.size
         assert n <= self._meta_cap
@@ -484,7 +554,10 @@ class Engine:
         for f in fields:
             views.append(self._meta_dev[off:off + len(f)])
             off += len(f)
-        (ctx.ids, ctx.tok_seq, ctx.tok_pos, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, ctx.want_rows) = views
+        (ctx.ids, ctx.tok_seq, ctx.tok_pos, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, ctx.want_rows) = views[:7]
+        ctx.prefix = groups
+        if groups is not None:
+            groups.bind(views[7])
         ctx.n_tokens, ctx.n_seqs, ctx.n_want = T, B, W
         ctx.max_new, ctx.max_len = max_new, max_len
         ctx.decode_only = False

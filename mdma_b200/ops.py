@@ -1168,6 +1168,14 @@ def prefix_split(tile_rows: int, blocks_wanted: int, tokens: int, seqs: int, max
     return pieces, max(1, min(blocks_wanted // own, 32, -(-most_own // 128)))
 
 
+def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int) -> tuple[int, int]:
+    """`prefix_split` for a step on the CUDA cores.  Of single tokens it follows from the most sequences the engine can hold,
+    not from the live ones, so that a request's sums are cut at the same places when a batch mate ends."""
+    one = ctx.max_new == 1
+    seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
+    return prefix_split(32, 4 * 148, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
+
+
 def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, pieces: int, own_splits: int, scratch, sinks, status,
                  sinks_log2: bool):
     """The arguments of the prefix attention kernels as one array (see csrc/prefix.cuh)."""
@@ -1217,10 +1225,7 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     if ctx.n_tokens == 0:
         return
     g = ctx.prefix
-    seqs = getattr(ctx, "most_seqs", None) or ctx.n_seqs
-    tokens = seqs if ctx.max_new == 1 else ctx.n_tokens
-    pieces, own = prefix_split(32, 4 * 148, tokens, seqs if ctx.max_new == 1 else ctx.n_seqs, ctx.max_new, g.most_len, g.most_own,
-                               n_heads, n_kv_heads)
+    pieces, own = prefix_plan(ctx, g, n_heads, n_kv_heads)
     need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.float32, device=q.device)

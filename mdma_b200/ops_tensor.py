@@ -638,6 +638,14 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
 
 
 # ---- attention of sequences that share their beginning (csrc/attention_prefix.cu) ------------------------------------------
+def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int) -> tuple[int, int]:
+    """(pieces of a prefix, pieces of a sequence's own keys); of single tokens from the most sequences the engine can hold (see
+    `ops.prefix_plan`)."""
+    one = ctx.max_new == 1
+    seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
+    return ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
+
+
 def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                      sink_log2: Optional[torch.Tensor] = None, st: Optional[TensorState] = None) -> None:
     """`ops.prefix_attention` in bfloat16 on the tensor cores (the geometries of `attention_supported`).  `sink_log2`: the sinks
@@ -653,10 +661,7 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     st = st or _device_state(q.device)
     flush_pending(q.device, st)
     g = ctx.prefix
-    seqs = getattr(ctx, "most_seqs", None) or ctx.n_seqs
-    one = ctx.max_new == 1
-    pieces, own = ops.prefix_split(64, 2 * st.sms, seqs if one else ctx.n_tokens, seqs if one else ctx.n_seqs, ctx.max_new, g.most_len,
-                                   g.most_own, n_heads, n_kv_heads)
+    pieces, own = prefix_plan(ctx, g, n_heads, n_kv_heads, st.sms)
     need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2)
     if own_st is not None:
         st.need(need, "attention over shared prefixes")

@@ -200,10 +200,14 @@ class Attention(Part):
                        self.v_dim, rotary_dim, interleaved, self.qk_norm_eps is not None, float(self.qk_norm_eps or 0.0),
                        owns_cache)
         gate = row[:, self.g_col:] if self.head_gate else None
-        if self._fast_ok:
+        shared = self._shares(ctx, view)
+        if shared:
+            self._attend_shared(ctx, row, view, out, self.sink_f32, self.sink_log2)
+        elif self._fast_ok:
             from .. import ops_tensor
             ops_tensor.attention(ctx, row, view, out, self.n_heads, self.n_kv_heads, self.head_dim, self.window,
                                  self.scale, st=self.rt.tc, sink_log2=self.sink_log2)
+        if shared or self._fast_ok:
             if gate is not None or self.out_scale != 1.0:
                 ops.head_gate(out, gate, n, self.n_heads, self.v_dim, self.out_scale)
         else:
@@ -234,7 +238,8 @@ class Attention(Part):
         qkv = ctx.buf("qkv", self.row_width)
         out = ctx.buf("attn_out", self.q_width)
         write = owns_cache and not self.shared_cache
-        if write and ctx.max_new == 1 and self._fast_ok and self._fusable(ctx, view):
+        shared = self._shares(ctx, view)
+        if write and not shared and ctx.max_new == 1 and self._fast_ok and self._fusable(ctx, view):
             # single tokens: the attention kernel rotates q and k and writes the cache itself
             from .. import ops_tensor
             inv_freq, rotary_dim, interleaved = self.position.rotary_table()
@@ -244,7 +249,9 @@ class Attention(Part):
             return out
         self.qkv_proj.store(h, qkv, n, defer=getattr(self.position, "fuses_pending", False))
         self.position.encode_and_store(ctx, qkv, self.n_heads, self.n_kv_heads, self.head_dim, view, write)
-        if self.rt.attention == "fast" and self._fast_ok:
+        if shared:
+            self._attend_shared(ctx, qkv, view, out)
+        elif self.rt.attention == "fast" and self._fast_ok:
             from .. import ops_tensor
             ops_tensor.attention(ctx, qkv, view, out, self.n_heads, self.n_kv_heads, self.head_dim,
                                  self.window, self.scale, st=self.rt.tc)
@@ -256,6 +263,38 @@ class Attention(Part):
                                  view.page_table, view.max_pages, view.page_size, out,
                                  self.n_heads, self.n_kv_heads, self.head_dim, self.window, self.scale)
         return out
+
+    def prefix_shapes(self) -> list:
+        """(heads, kv heads, head size) of the attention that may run over shared prefixes: its keys stay in sight."""
+        return [(self.n_heads, self.n_kv_heads, self.head_dim)] if not self.window and self.v_dim == self.head_dim else []
+
+    def _shares(self, ctx, view) -> bool:
+        """Whether this step's attention reads shared prefixes once: sequences of the step have forked from one another, every key stays
+        in sight, and the parts fit the engine's scratch (steps of many tokens a sequence run without: their tiles are full,
+        whoever shares)."""
+        g = getattr(ctx, "prefix", None)
+        if g is None or view.window or not self.prefix_shapes():
+            return False
+        if self._fast_ok:
+            from .. import ops_tensor
+            if ctx.max_new * (self.n_heads // self.n_kv_heads) > 64:
+                return False
+            parts = sum(ops_tensor.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads, self.rt.tc.sms if self.rt.tc is not None else 148))
+            scratch = self.rt.tc.scratch if self.rt.tc is not None and not self.rt.tc.growable else None
+        else:
+            parts, scratch = sum(ops.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads)), self.rt.prefix_scratch
+        return scratch is None or ctx.n_tokens * self.n_heads * parts * (self.head_dim + 2) <= scratch.numel()
+
+    def _attend_shared(self, ctx, row, view, out, sinks=None, sinks_log2=None):
+        sizes = (self.n_heads, self.n_kv_heads, self.head_dim, self.scale)
+        if self._fast_ok:
+            from .. import ops_tensor
+            ops_tensor.prefix_attention(ctx, row, view, out, *sizes, sink_log2=sinks_log2, st=self.rt.tc)
+            return
+        if self.rt.gemm == "tensor":
+            from .. import ops_tensor
+            ops_tensor.flush_pending(row.device, self.rt.tc)
+        ops.prefix_attention(ctx, row, view, out, *sizes, sinks=sinks, scratch=self.rt.prefix_scratch)
 
     def _fusable(self, ctx, view) -> bool:
         """Whether this step's attention kernel should do the position encoding and the cache write

@@ -34,6 +34,7 @@ class Runtime:
     gemm: str = "simt"                 # "simt" | "tensor" (tcgen05; bfloat16 only)
     attention: str = "simple"          # "simple" | "fast"
     tc: object = None                  # the engine's `ops_tensor.TensorState` (None: a shared default)
+    prefix_scratch: object = None      # the engine's floats for the parts of attention over shared prefixes (None: per call)
     alloc: object = None               # alloc(shape, dtype) for the device tensors a part derives at bind
 
     def unfolded(self, run, *args):
