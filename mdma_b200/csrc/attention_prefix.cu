@@ -1,5 +1,9 @@
 // Attention over shared prefixes on the tensor cores (bfloat16 in, float softmax and accumulation).  See prefix.cuh for the
 // parts and how they join.
+#include <mutex>
+
+#include "attention_prefix_own.cuh"
+#include "attention_prefix_tc.cuh"
 #include "mma_tiles.cuh"
 #include "prefix.cuh"
 
@@ -19,8 +23,9 @@ prefix_rows_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
     __shared__ int row_token[kPrRows];
     const uint32_t sQ = (uint32_t)__cvta_generic_to_shared(smem), sK = sQ + kTile, sV = sK + 2 * kTile;
 
-    chain_release();
     chain_wait();
+    // only now: a kernel that starts early behind this one may count on what this one waited for
+    chain_release();
     const int G = p.group, D = p.head_dim, kvh = blockIdx.y, tt = kPrRows / G, split = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool prefix = (int)blockIdx.x < prefix_tiles;
@@ -158,10 +163,18 @@ prefix_rows_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
     }
 }
 
-static int launch_prefix_rows(const PrefixParams& p, cudaStream_t stream) {
+static int launch_prefix_merge(const PrefixParams& p, cudaStream_t stream) {
+    const long rows = (long)p.n_tokens * p.n_heads;
+    const cudaError_t e = launch_chained(prefix_merge_kernel<__nv_bfloat16>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, p);
+    if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+// The prefixes, the sequences' own keys, or both.
+static int launch_prefix_rows(const PrefixParams& p, bool prefixes, bool own, cudaStream_t stream) {
     const int tt = kPrRows / p.group, own_tiles = (p.max_new + tt - 1) / tt;
-    const long prefix_tiles = prefix_tiles_bound(p, tt), tiles = prefix_tiles + (long)own_tiles * p.n_seqs;
-    const int splits = p.pieces > p.own_splits ? p.pieces : p.own_splits;
+    const long prefix_tiles = prefixes ? prefix_tiles_bound(p, tt) : 0, tiles = prefix_tiles + (own ? (long)own_tiles * p.n_seqs : 0);
+    const int splits = prefixes && (!own || p.pieces > p.own_splits) ? p.pieces : p.own_splits;
     MDMA_REQUIRE(tiles <= 0x7fffffffl && p.n_kv_heads <= 65535 && splits <= 65535, "prefix_attention: grid too large");
     auto run = [&](auto kernel, int dmax) -> int {
         const int bytes = 5 * kPrRows * dmax * 2;
@@ -170,9 +183,70 @@ static int launch_prefix_rows(const PrefixParams& p, cudaStream_t stream) {
         if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
         return 0;
     };
-    if (int rc = p.head_dim <= 64 ? run(prefix_rows_kernel<64>, 64) : run(prefix_rows_kernel<128>, 128)) return rc;
-    const long rows = (long)p.n_tokens * p.n_heads;
-    const cudaError_t e = launch_chained(prefix_merge_kernel<__nv_bfloat16>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, p);
+    return p.head_dim <= 64 ? run(prefix_rows_kernel<64>, 64) : run(prefix_rows_kernel<128>, 128);
+}
+
+// A tensor map over a cache [pages, page_size, kv_heads, head_dim] with boxes of 64 numbers x 1 head x `keys` keys x 1 page
+// (128-byte swizzle).
+typedef CUresult (*PrefixEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static int prefix_cache_map(CUtensorMap* out, const void* cache, const PrefixParams& p, int keys) {
+    static PrefixEncodeFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PrefixEncodeFn>(sym);
+    });
+    if (!fn) return fail("prefix_attention: the driver does not offer cuTensorMapEncodeTiled");
+    const cuuint64_t row = (cuuint64_t)p.n_kv_heads * p.head_dim * 2;
+    cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.page_size, (cuuint64_t)p.n_pages};
+    cuuint64_t strides[3] = {(cuuint64_t)p.head_dim * 2, row, row * p.page_size};
+    cuuint32_t box[4] = {64, 1, (cuuint32_t)keys, 1}, elem[4] = {1, 1, 1, 1};
+    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(cache), dims, strides, box, elem,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("prefix_attention: cuTensorMapEncodeTiled failed with %d", (int)r);
+    return 0;
+}
+
+static bool prefix_own_fits(const PrefixParams& p) {
+    return p.max_new == 1 && p.group <= 16 && p.page_size % 32 == 0 && p.pieces <= kPoMaxPieces && p.own_splits >= 1;
+}
+static int launch_prefix_own(const PrefixParams& p, int sms, cudaStream_t stream) {
+    const int kb = p.head_dim <= 64 && p.page_size % 64 == 0 ? 64 : 32;       // a tile of 8 KB either way
+    const long blocks = (long)p.n_kv_heads * p.own_splits * p.n_seqs;
+    MDMA_REQUIRE(p.n_seqs <= 65535 && blocks <= 0x7fffffffl, "prefix_attention: grid too large");
+    CUtensorMap mk, mv;
+    if (int rc = prefix_cache_map(&mk, p.k_cache, p, kb)) return rc;
+    if (int rc = prefix_cache_map(&mv, p.v_cache, p, kb)) return rc;
+    auto run = [&](auto kernel, int nw, int bytes) -> int {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) e = launch_chained(kernel, dim3(p.n_kv_heads * p.own_splits, p.n_seqs), dim3(nw * 32), bytes, stream, mk, mv, p);
+        if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
+        return 0;
+    };
+    // the most warps a block with which every block is resident at once; rounds of four-warp blocks where there are too many
+    const int nw = blocks <= sms ? 12 : blocks <= 3l * sms ? 4 : blocks <= 5l * sms ? 2 : blocks <= 10l * sms ? 1 : 4;
+#define MDMA_OWN(DM, KB) (nw == 12 ? run(prefix_own_kernel<DM, KB, 12>, 12, PoSmem<DM, KB, 12>::kBytes) \
+                        : nw == 4 ? run(prefix_own_kernel<DM, KB, 4>, 4, PoSmem<DM, KB, 4>::kBytes) \
+                        : nw == 2 ? run(prefix_own_kernel<DM, KB, 2>, 2, PoSmem<DM, KB, 2>::kBytes) \
+                                  : run(prefix_own_kernel<DM, KB, 1>, 1, PoSmem<DM, KB, 1>::kBytes))
+    return kb == 64 ? MDMA_OWN(64, 64) : p.head_dim <= 64 ? MDMA_OWN(64, 32) : MDMA_OWN(128, 32);
+#undef MDMA_OWN
+}
+
+static int launch_prefix_tc(const PrefixParams& p, cudaStream_t stream) {
+    const long tiles = prefix_tiles_bound(p, 2 * (kPtRows / p.group));
+    MDMA_REQUIRE(tiles <= 65535 && p.pieces <= 65535, "prefix_attention: grid too large");
+    CUtensorMap mk, mv;
+    if (int rc = prefix_cache_map(&mk, p.k_cache, p, 64)) return rc;
+    if (int rc = prefix_cache_map(&mv, p.v_cache, p, 64)) return rc;
+    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPtSmem);
+    if (e == cudaSuccess) e = launch_chained(prefix_tc_kernel, dim3(p.n_kv_heads, (unsigned)tiles, p.pieces), dim3(kPtThreads), kPtSmem, stream, mk, mv, p);
     if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }
@@ -189,6 +263,24 @@ extern "C" int mdma_prefix_attention(const long long* words, int n_words, float 
                  p.n_heads, p.n_kv_heads, p.head_dim);
     MDMA_REQUIRE(p.q_stride % 8 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache) & 15) == 0, "prefix_attention: rows must be 16-byte aligned");
     MDMA_REQUIRE(((uintptr_t)p.part_o & 15) == 0, "prefix_attention: the scratch must be 16-byte aligned");
+    MDMA_REQUIRE(((uintptr_t)p.out & 15) == 0, "prefix_attention: the results must be 16-byte aligned");
+    const bool tiled = p.page_size % 64 == 0;
+    MDMA_REQUIRE(!p.whole || tiled, "prefix_attention: whole lists of keys want pages of a multiple of 64 tokens");
     if (p.n_tokens == 0 || p.n_seqs == 0) return 0;
-    return launch_prefix_rows(p, stream);
+    if (tiled) {
+        if (int rc = launch_prefix_tc(p, stream)) return rc;
+        if (p.whole && p.pieces == 1) return 0;
+    }
+    if (!p.whole && prefix_own_fits(p)) {
+        if (!tiled)
+            if (int rc = launch_prefix_rows(p, true, false, stream)) return rc;
+        int sms = 0, dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            return fail("prefix_attention: no CUDA device");
+        if (int rc = launch_prefix_own(p, sms, stream)) return rc;
+        if (p.own_splits == 1) return 0;
+    } else if (!p.whole) {
+        if (int rc = launch_prefix_rows(p, !tiled, true, stream)) return rc;
+    }
+    return launch_prefix_merge(p, stream);
 }

@@ -34,7 +34,8 @@ LIBRARIES = {
              ["common.cuh", "ptx.cuh", "delta_rule.cuh", "float4.cuh", "rows_product.cuh", "linear_input.cuh", "prefix.cuh"], []),
     "tensor": (["gemm_tcgen05.cu", "attention_mma.cu", "attention_tc.cu", "attention_talking_mma.cu",
                 "attention_mixed_weights_mma.cu", "attention_prefix.cu"],
-               ["common.cuh", "ptx.cuh", "attention_mma.cuh", "mma_tiles.cuh", "prefix.cuh"], []),
+               ["common.cuh", "ptx.cuh", "attention_mma.cuh", "mma_tiles.cuh", "prefix.cuh",
+                "attention_prefix_tc.cuh", "attention_prefix_own.cuh"], []),
     "noalloc": (["attention_noalloc.cu"], ["common.cuh", "ptx.cuh", "attention_mma.cuh", "mma_tiles.cuh", "attention_noalloc.h"], []),
 }
 

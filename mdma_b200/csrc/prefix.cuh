@@ -23,6 +23,7 @@ struct PrefixParams {
     int n_groups, n_seqs, n_tokens, max_new;
     int n_heads, n_kv_heads, head_dim, group;
     int pieces, own_splits;                          // a prefix in `pieces` pieces at most, own keys in `own_splits`: slots of the parts
+    int whole;                                       // own_splits 0: all keys of a row tile, prefix and own ones, are one list in `pieces` pieces
     float scale_log2;                                // scale * log2(e)
     const float* sinks; float sink_rate;             // sinks[head] * sink_rate is in powers of two; null: none
     int* status;
@@ -40,11 +41,11 @@ __host__ __device__ __forceinline__ int prefix_pieces_used(int len, int pieces) 
 }
 
 // Tile t of the prefixes' query rows, `tile_tokens` tokens each: which group, which of its tokens.  Groups without a prefix
-// have no tiles.  False: there is no such tile.
+// have no tiles (unless their own keys are walked, too).  False: there is no such tile.
 struct PrefixTile { int g, first, count; };          // toks[first .. first + count)
 __device__ __forceinline__ bool prefix_tile(const PrefixParams& p, int t, int tile_tokens, PrefixTile& out) {
     for (int g = 0; g < p.n_groups; ++g) {
-        if (p.group_len[g] <= 0) continue;
+        if (p.group_len[g] <= 0 && !p.whole) continue;
         const int a = p.tok_first[g], n = p.tok_first[g + 1] - a, tiles = (n + tile_tokens - 1) / tile_tokens;
         if (t < tiles) {
             out.g = g; out.first = a + t * tile_tokens; out.count = min(tile_tokens, n - t * tile_tokens);
@@ -69,7 +70,7 @@ prefix_merge_kernel(const PrefixParams p) {
     const int lane = threadIdx.x & 31;
     if (row >= (long)p.n_tokens * p.n_heads) return;
     const int slots = p.pieces + p.own_splits, D = p.head_dim;
-    const int used = prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces);
+    const int used = p.whole ? p.pieces : prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces);
     const float* ml = p.part_ml + row * slots * 2;
     float m = -INFINITY;
     for (int s = 0; s < used + p.own_splits; ++s) m = fmaxf(m, ml[2 * (s < used ? s : p.pieces + s - used)]);
@@ -121,11 +122,12 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     MDMA_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0, "prefix_attention: %d heads over %d kv heads", p.n_heads, p.n_kv_heads);
     MDMA_REQUIRE(p.head_dim > 0 && p.head_dim <= 256, "prefix_attention: head_dim %d is beyond the limit of 256", p.head_dim);
     MDMA_REQUIRE(p.page_table && p.page_size > 0 && p.max_pages > 0, "prefix_attention: bad cache geometry");
-    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 1 && p.own_splits >= 1, "prefix_attention: bad sizes");
+    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 1 && p.own_splits >= 0, "prefix_attention: bad sizes");
     MDMA_REQUIRE(scale > 0.f, "prefix_attention: the score scale must be positive");
     p.group = p.n_heads / p.n_kv_heads;
-    const long long slots = (long long)p.n_tokens * p.n_heads * (p.pieces + p.own_splits), need = slots * (p.head_dim + 2);
-    MDMA_REQUIRE(scratch && floats >= need, "prefix_attention: %lld floats of scratch are needed, %lld given", need, floats);
+    p.whole = p.own_splits == 0;
+    const long long slots = p.whole && p.pieces == 1 ? 0 : (long long)p.n_tokens * p.n_heads * (p.pieces + p.own_splits), need = slots * (p.head_dim + 2);
+    MDMA_REQUIRE(need == 0 || (scratch && floats >= need), "prefix_attention: %lld floats of scratch are needed, %lld given", need, floats);
     p.part_o = scratch; p.part_ml = scratch + slots * p.head_dim;
     return 0;
 }

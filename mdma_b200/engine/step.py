@@ -127,7 +127,7 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
     if dtype == torch.bfloat16:
         from .. import ops_tensor
         floats = ops_tensor.scratch_floats_bound(sms, chunk_tokens, max_slots, shapes)
-    floats = max(floats, prefix_floats(model, dtype, sms, max_slots, max_context))
+    floats = max(floats, prefix_floats(model, dtype, sms, max_slots, max_context, page_size))
     lay.scratch_floats = floats
     lay.tc_sk_flags = carver.take("kernel_scratch", (max(512, 4 * sms),), torch.int32)
     lay.tc_scratch = carver.take("kernel_scratch", (max(floats, 1),), torch.float32)
@@ -135,7 +135,7 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
     return lay
 
 
-def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_context: int) -> int:
+def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_context: int, page_size: int) -> int:
     """Scratch for single-token steps over shared prefixes: the parts of every sequence's softmaxes (steps of several tokens
     use it as far as it goes)."""
     from types import SimpleNamespace
@@ -148,7 +148,7 @@ def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_cont
         for heads, kv_heads, head_dim in getattr(part, "prefix_shapes", list)():
             parts = sum(ops.prefix_plan(ctx, most, heads, kv_heads))
             if dtype == torch.bfloat16 and ops_tensor.attention_supported(heads, kv_heads, head_dim):
-                parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, sms)))
+                parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, sms, page_size)))
             need = max(need, max_slots * heads * parts * (head_dim + 2))
     return need
 

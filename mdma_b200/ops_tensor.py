@@ -638,11 +638,31 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
 
 
 # ---- attention of sequences that share their beginning (csrc/attention_prefix.cu) ------------------------------------------
-def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int) -> tuple[int, int]:
+def prefix_own_splits(seqs: int, n_heads: int, n_kv_heads: int, most_own: int, sms: int) -> int:
+    """Into how many pieces a single token's own keys are cut: one block a (sequence, kv head) joins everything itself unless
+    the blocks leave most of the device idle and have more than a thousand keys each."""
+    if n_heads // n_kv_heads > 16:
+        return ops.prefix_split(64, 2 * sms, seqs, seqs, 1, 0, most_own, n_heads, n_kv_heads)[1]
+    if seqs * n_kv_heads * 2 > sms or most_own <= 1024:
+        return 1
+    return max(1, min(sms // (seqs * n_kv_heads), most_own // 512, 16))
+
+
+def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int, page_size: int) -> tuple[int, int]:
     """(pieces of a prefix, pieces of a sequence's own keys); of single tokens from the most sequences the engine can hold (see
-    `ops.prefix_plan`)."""
+    `ops.prefix_plan`).  (n, 0): prefix and own keys are one list in n pieces."""
     one = ctx.max_new == 1
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
+    if page_size % 64 == 0:                       # the tcgen05 kernel: 256 query rows a block, one block an SM
+        tile_tokens = 2 * (128 // (n_heads // n_kv_heads))
+        tiles = -(-seqs // tile_tokens) if one else ctx.n_tokens // tile_tokens + g.n_groups
+        most = sms // (tiles * n_kv_heads)
+        if not one:
+            return max(1, min(most, 32, (g.most_len + g.most_own) // 256)), 0
+        return max(1, min(most, 32, -(-g.most_len // 128))), prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms)
+    if one and page_size % 32 == 0 and n_heads // n_kv_heads <= 16:
+        return (ops.prefix_split(64, 2 * sms, seqs, seqs, 1, g.most_len, 0, n_heads, n_kv_heads)[0],
+                prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms))
     return ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
 
 
@@ -661,8 +681,8 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     st = st or _device_state(q.device)
     flush_pending(q.device, st)
     g = ctx.prefix
-    pieces, own = prefix_plan(ctx, g, n_heads, n_kv_heads, st.sms)
-    need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2)
+    pieces, own = prefix_plan(ctx, g, n_heads, n_kv_heads, st.sms, view.page_size)
+    need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2) if pieces + own > 1 else 0
     if own_st is not None:
         st.need(need, "attention over shared prefixes")
         scratch = st.scratch

@@ -270,16 +270,16 @@ class Attention(Part):
 
     def _shares(self, ctx, view) -> bool:
         """Whether this step's attention reads shared prefixes once: sequences of the step have forked from one another, every key stays
-        in sight, and the parts fit the engine's scratch (steps of many tokens a sequence run without: their tiles are full,
-        whoever shares)."""
+        in sight, and the parts fit the engine's scratch."""
         g = getattr(ctx, "prefix", None)
         if g is None or view.window or not self.prefix_shapes():
             return False
         if self._fast_ok:
             from .. import ops_tensor
-            if ctx.max_new * (self.n_heads // self.n_kv_heads) > 64:
-                return False
-            parts = sum(ops_tensor.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads, self.rt.tc.sms if self.rt.tc is not None else 148))
+            parts = sum(ops_tensor.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads, self.rt.tc.sms if self.rt.tc is not None else 148,
+                                               view.page_size))
+            if parts == 1:
+                return True
             scratch = self.rt.tc.scratch if self.rt.tc is not None and not self.rt.tc.growable else None
         else:
             parts, scratch = sum(ops.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads)), self.rt.prefix_scratch

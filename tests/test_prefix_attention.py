@@ -47,6 +47,7 @@ BATCHES = [
     ("groups and loners", [(300, ONE), (0, [(20, 1)]), (7, [(0, 1), (200, 1)]), (0, [(0, 1)]), (64, [(3, 1)])]),
     ("more rows than a tile", [(200, [(i % 5, 1) for i in range(70)])]),
     ("a long prefix, own keys of all lengths", [(1500, [(i * 37 % 400, 1) for i in range(6)])]),
+    ("own keys beyond a thousand", [(70, [(1500, 1), (3, 1)]), (0, [(1100, 1)])]),
     ("short prompts", [(131, [(0, 3), (0, 17), (9, 1), (0, 40)])]),
     ("prompts longer than the prefix", [(10, [(0, 150), (3, 77)]), (0, [(0, 130)]), (0, [(5, 2)])]),
     ("prompts and single tokens", [(260, [(0, 1), (0, 65), (129, 1)]), (513, [(0, 9), (1, 64)])]),
