@@ -4,13 +4,20 @@
 // several members of a group, and walks a list of key blocks of 128:
 //     S = Q K^T    tcgen05.mma, M = N = 128, operands from shared memory (keys by TMA, 128-byte swizzle), S in tensor memory
 //     softmax      128 threads a tile, a row a thread: the row out of tensor memory, mask, running maximum and sum in float, the
-//                  weights rounded to bfloat16 and written back over S
-//     O += P V     tcgen05.mma, A = P from tensor memory, V as the cache holds it (MN-major), O in tensor memory
+//                  weights rounded to bfloat16 and written back over S, 64 keys at a time
+//     O += P V     tcgen05.mma, A = P from tensor memory, V as the cache holds it (MN-major), O in tensor memory; the first 64
+//                  keys' product runs under the second's exponentials
 // The two tiles take turns: while one is in its softmax the tensor pipe works for the other, and both use the same key and
-// value blocks.  Tensor memory: S and P of the tiles in columns 0 and 128, O in 256 and 384.  The products of a tile are issued by one thread
-// in the order S(0), P(0) V(0), S(1), .., so whoever sees S(j) complete knows that P(j-1) V(j-1) is, too.
+// value blocks.  Tensor memory: S and P of the tiles in columns 0 and 128, O in 256 and 384.  One thread issues all products, a
+// tile's P V and its next S one behind the other, so whoever sees S(j) complete knows that P(j-1) V(j-1) is, too, and the
+// tiles' S are complete half a period apart.
 // The weights are taken against a reference that moves only when a row's maximum has grown by more than 2^8 since; O is
-// rescaled only then.
+// rescaled only then.  Of every four exponentials one goes through a polynomial on the multiply-add units (`exp2_poly`), which
+// the exponential unit (16 results a cycle and SM) would be the bound of otherwise.
+// Measured, cycles a block of 128 keys and both tiles (the tensor pipe's own: 2,048): 3,400.  What was slower: two threads a row
+// (the issue slots of sixteen softmax warps are the bound then) 4,200; a warp that issues for each tile, both in step, 4,850; P V
+// behind the whole softmax 3,450; steps of 64 keys with two places for S (products of N = 64 cost as much as of N = 128) 3,700.
+// 8,960 rows a kv head over 8,000 keys, 32 heads of 128: 321 us, 996 TFLOP/s.
 //
 // The list: the prefix's blocks, which all rows see, and (`whole`) behind them the own blocks of every sequence with tokens in the
 // tiles, which only that sequence's rows see: the others' lanes of O are left out of the product, so that what they are
@@ -29,31 +36,64 @@ struct PtSegment { int seq, key0, key1, tok0, toks, block0; };  // keys [key0, k
 constexpr int kPtSmemSegs = kPtSmemBars + 256;
 constexpr int kPtSmem = kPtSmemSegs + (kPtMaxTokens + 4) * (int)sizeof(PtSegment);
 
-// Walks the blocks of a list.
+// Walks the blocks of a list; what the current segment says is kept in registers.
 struct PtWalk {
     const PtSegment* segs;
-    int seg, block;
-    __device__ __forceinline__ PtWalk(const PtSegment* s, int first) : segs(s), seg(0), block(first) {
+    int seg, block, next0;                                       // the segment, the block of the list, the next segment's first block
+    PtSegment s;
+    int key;                                                     // the block's first key (of an own segment's first block: the multiple of 64 below its first key)
+    int ra[2], rb[2];                                            // rows [ra, rb) of each tile see the block
+    __device__ __forceinline__ PtWalk(const PtSegment* list, int first, int tt, int G) : segs(list), seg(0), block(first) {
         while (first >= segs[seg + 1].block0) ++seg;
+        enter(tt, G);
+        key += (block - s.block0) * kPtKeys;
     }
-    __device__ __forceinline__ void next() {
-        ++block;
-        while (block >= segs[seg + 1].block0) ++seg;
+    __device__ __forceinline__ void enter(int tt, int G) {
+        s = segs[seg];
+        next0 = segs[seg + 1].block0;
+        key = s.key0 & ~63;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            ra[t] = max(s.tok0 - t * tt, 0) * G;
+            rb[t] = max(min(s.tok0 + s.toks - t * tt, tt), 0) * G;
+        }
     }
-    __device__ __forceinline__ const PtSegment& s() const { return segs[seg]; }
-    // (of an own segment the first block starts at the multiple of 64 below its first key)
-    __device__ __forceinline__ int key() const { return (s().key0 & ~63) + (block - s().block0) * kPtKeys; }
-    // rows [a, b) of tile `tile` that see this block
-    __device__ __forceinline__ void rows(int tile, int tt, int G, int& a, int& b) const {
-        a = max(s().tok0 - tile * tt, 0) * G;
-        b = max(min(s().tok0 + s().toks - tile * tt, tt), 0) * G;
+    __device__ __forceinline__ void next(int tt, int G) {
+        key += kPtKeys;
+        if (++block < next0) return;
+        do ++seg; while (block >= segs[seg + 1].block0);
+        enter(tt, G);
     }
-    __device__ __forceinline__ bool active(int tile, int tt, int G) const {
-        int a, b;
-        rows(tile, tt, G, a, b);
-        return a < b;
-    }
+    __device__ __forceinline__ bool active(int t) const { return ra[t] < rb[t]; }
+    __device__ __forceinline__ int steps() const { return s.key1 - key > 64 ? 2 : 1; }        // of 64 keys
 };
+
+// 2^x for x <= 126 by range reduction to [-1/2, 1/2] and a polynomial (minimax in the relative error, 2.7e-6; own fit); two at
+// once.  The sum with 1.5 2^23 leaves the nearest integer in the low bits, which move into the exponent.
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    const float magic = 12582912.0f;
+    x.x = fmaxf(x.x, -126.0f); x.y = fmaxf(x.y, -126.0f);
+    const float2 t = add_pair(x, make_float2(magic, magic));
+    const float2 n = add_pair(t, make_float2(-magic, -magic));
+    const float2 f = fma_pair(n, make_float2(-1.f, -1.f), x);
+    float2 y = fma_pair(f, make_float2(0.009570102207362652f, 0.009570102207362652f), make_float2(0.05591785907745361f, 0.05591785907745361f));
+    y = fma_pair(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    y = fma_pair(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    y = fma_pair(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
 
 __global__ void __launch_bounds__(kPtThreads, 1)
 prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams p) {
@@ -64,23 +104,38 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     auto v_full = [&](int s) { return bars + 8u * (4 + s); };
     auto v_empty = [&](int s) { return bars + 8u * (6 + s); };
     auto s_full = [&](int t) { return bars + 8u * (8 + t); };
-    auto p_ready = [&](int t) { return bars + 8u * (10 + t); };
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kPtSmemBars + 8 * 12);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kPtSmemBars + 8 * 13);
-    int* warp_starts = reinterpret_cast<int*>(smem + kPtSmemBars + 8 * 14);          // [9]
+    auto p_ready = [&](int t, int half) { return bars + 8u * (10 + 2 * t + half); };
+    const uint32_t q_full = bars + 8u * 14;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kPtSmemBars + 8 * 15);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kPtSmemBars + 8 * 16);
+    int* warp_starts = reinterpret_cast<int*>(smem + kPtSmemBars + 8 * 17);          // [9]
     PtSegment* segs = reinterpret_cast<PtSegment*>(smem + kPtSmemSegs);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.group, D = p.head_dim, kvh = blockIdx.x, split = blockIdx.z, tt = kPtRows / G;
 
     chain_wait();
+    // ---- which rows, which keys ------------------------------------------------------------------------------------
     PrefixTile tile;
     if (!prefix_tile(p, blockIdx.y, 2 * tt, tile)) return;
+    const int count = tile.count, len = tile.len;                // tokens of both tiles; the prefix
+    int b0 = 0, b1 = 0;                                          // this block's part of the list
+    if (!p.whole) {
+        const int keys = prefix_piece(len, p.pieces), lo = split * keys, hi = min(len, lo + keys);
+        if (lo >= hi) return;
+        if (threadIdx.x == 0) {
+            segs[0] = {p.group_seq[tile.g], lo, hi, 0, count, 0};
+            segs[1].block0 = 0x7fffffff;
+        }
+        b1 = (hi - lo + kPtKeys - 1) / kPtKeys;
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(k_full(s), 1); ptx::mbar_init(k_empty(s), 1);
             ptx::mbar_init(v_full(s), 1); ptx::mbar_init(v_empty(s), 1);
-            ptx::mbar_init(s_full(s), 1); ptx::mbar_init(p_ready(s), 128);
+            ptx::mbar_init(s_full(s), 1);
+            for (int h = 0; h < 2; ++h) ptx::mbar_init(p_ready(s, h), 4);        // a tile's four warps
         }
+        ptx::mbar_init(q_full, 256);
         *abort_flag = (base & 1023u) ? 1 : 0;                    // the tiles need 1024-byte alignment
         ptx::fence_mbar_init();
     }
@@ -91,85 +146,54 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint32_t tmem = *tmem_slot;
     // only now: a kernel that starts early behind this one may count on what this one waited for, and finds the tensor memory taken
     chain_release();
-
-    // ---- which rows, which keys ------------------------------------------------------------------------------------
-    const bool found = !(base & 1023u);
-    const int count = tile.count;                                // tokens of both tiles
-    int blocks = 0, b0 = 0, b1 = 0;
-    if (found) {                                                 // (uniform over the block)
-        const int len = p.group_len[tile.g];
-        if (!p.whole) {
-            const int keys = prefix_piece(len, p.pieces), lo = split * keys, hi = min(len, lo + keys);
-            if (threadIdx.x == 0) {
-                segs[0] = {p.group_seq[tile.g], lo, hi, 0, count, 0};
-                segs[1].block0 = 0x7fffffff;
-            }
-            b1 = blocks = hi > lo ? (hi - lo + kPtKeys - 1) / kPtKeys : 0;
-        } else {
-            // a segment starts where the token's sequence differs from that of the token before
-            const int t = threadIdx.x;
-            int token = 0, seq = -1, before = -1;
-            if (t < count) {
-                token = p.toks[tile.first + t]; seq = p.tok_seq[token];
-                before = t > 0 ? p.tok_seq[p.toks[tile.first + t - 1]] : -1;
-            }
-            const bool starts = t < count && seq != before;
-            const uint32_t mask = __ballot_sync(0xffffffffu, starts);
-            if (warp < 8 && lane == 0) warp_starts[warp] = __popc(mask);
-            __syncthreads();
-            const int shared = len > 0 ? 1 : 0;
-            if (starts) {
-                int at = shared + __popc(mask & ((1u << lane) - 1u));
-                for (int w = 0; w < warp; ++w) at += warp_starts[w];
-                const int first = p.seq_start[seq], n = min(p.seq_start[seq + 1] - token, count - t);
-                segs[at] = {seq, p.seq_skip[seq], p.seq_pos0[seq] + token - first + n, t, n, 0};
-            }
-            if (threadIdx.x == 0 && shared) segs[0] = {p.group_seq[tile.g], 0, len, 0, count, 0};
-            __syncthreads();
-            int n_segs = shared;
+    if (p.whole) {
+        // a segment starts where the token's sequence differs from that of the token before
+        const int t = threadIdx.x;
+        int token = 0, seq = -1, before = -1;
+        if (t < count) {
+            token = p.toks[tile.first + t]; seq = p.tok_seq[token];
+            before = t > 0 ? p.tok_seq[p.toks[tile.first + t - 1]] : -1;
+        }
+        const bool starts = t < count && seq != before;
+        const uint32_t mask = __ballot_sync(0xffffffffu, starts);
+        if (warp < 8 && lane == 0) warp_starts[warp] = __popc(mask);
+        __syncthreads();
+        const int shared = len > 0 ? 1 : 0;
+        if (starts) {
+            int at = shared + __popc(mask & ((1u << lane) - 1u));
+            for (int w = 0; w < warp; ++w) at += warp_starts[w];
+            const int first = p.seq_start[seq], n = min(p.seq_start[seq + 1] - token, count - t);
+            segs[at] = {seq, p.seq_skip[seq], p.seq_pos0[seq] + token - first + n, t, n, 0};
+        }
+        if (threadIdx.x == 0 && shared) segs[0] = {p.group_seq[tile.g], 0, len, 0, count, 0};
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int n_segs = shared, at = 0;
             for (int w = 0; w < 8; ++w) n_segs += warp_starts[w];
-            if (threadIdx.x == 0) {
-                int at = 0;
-                for (int s = 0; s < n_segs; ++s) {
-                    segs[s].block0 = at;
-                    at += max(segs[s].key1 - (segs[s].key0 & ~63) + kPtKeys - 1, 0) / kPtKeys;
-                }
-                segs[n_segs].block0 = at;
-                segs[n_segs + 1].block0 = 0x7fffffff;
-                warp_starts[8] = at;
+            for (int s = 0; s < n_segs; ++s) {
+                segs[s].block0 = at;
+                at += max(segs[s].key1 - (segs[s].key0 & ~63) + kPtKeys - 1, 0) / kPtKeys;
             }
-            __syncthreads();
-            blocks = warp_starts[8];
-            const int per = (blocks + p.pieces - 1) / p.pieces;
-            b0 = split * per; b1 = min(blocks, b0 + per);
+            segs[n_segs].block0 = at;
+            segs[n_segs + 1].block0 = 0x7fffffff;
+            warp_starts[8] = at;
         }
-        // queries into shared memory, 128-byte rows with the 128-byte swizzle, zeros beyond the tiles' rows
-        if (b0 < b1 && warp < 8) {
-            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q);
-            const int chunks = ((D + 63) / 64) * 8;
-            for (int i = threadIdx.x; i < 2 * kPtRows * chunks; i += 256) {
-                const int r = i / chunks, c = i % chunks, tr = r % kPtRows, t = r / kPtRows * tt + tr / G;
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (tr / G < tt && t < count && c * 8 < D)
-                    x = *reinterpret_cast<const uint4*>(q + (size_t)p.toks[tile.first + t] * p.q_stride + (size_t)(kvh * G + tr % G) * D + c * 8);
-                *reinterpret_cast<uint4*>(smem + r / kPtRows * kPtSlot + (c >> 3) * kPtHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = x;
-            }
-            ptx::fence_proxy_async_shared();
-        }
+        __syncthreads();
+        const int blocks = warp_starts[8], per = (blocks + p.pieces - 1) / p.pieces;
+        b0 = split * per; b1 = min(blocks, b0 + per);
     }
-    __syncthreads();
-    const bool working = b0 < b1;
+    const bool working = b0 < b1 && !(base & 1023u);
     const int halves = (D + 63) / 64;
 
     if (working && warp == 8 && lane == 0) {
         // ---- TMA producer: K(0) V(0) K(1) V(1) .. -----------------------------------------------------------------
-        PtWalk w(segs, b0);
+        PtWalk w(segs, b0, tt, G);
         bool fine = true;
-        for (int j = 0; fine && b0 + j < b1; ++j, w.next()) {
-            const int* pages = p.page_table + (size_t)p.seq_slot[w.s().seq] * p.max_pages;
-            const int key0 = w.key(), boxes = w.s().key1 - key0 > 64 ? 2 : 1;       // of 64 keys each
+        for (int j = 0; fine && b0 + j < b1; ++j, w.next(tt, G)) {
+            const int* pages = p.page_table + (size_t)p.seq_slot[w.s.seq] * p.max_pages;
+            const int boxes = w.steps();                         // of 64 keys each
             int page[2], row[2];
-            for (int b = 0; b < boxes; ++b) { page[b] = pages[(key0 + 64 * b) / p.page_size]; row[b] = (key0 + 64 * b) % p.page_size; }
+            for (int b = 0; b < boxes; ++b) { page[b] = pages[(w.key + 64 * b) / p.page_size]; row[b] = (w.key + 64 * b) % p.page_size; }
             const int s = j & 1;
             const uint32_t phase = ((j >> 1) & 1) ^ 1;
             for (int which = 0; which < 2 && fine; ++which) {
@@ -183,19 +207,23 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                          full, h * 64, kvh, row[b], page[b]);
             }
         }
-    } else if (working && warp == 9 && lane == 0) {
-        // ---- MMA issuer ---------------------------------------------------------------------------------------------
+    } else if (working && warp == 9) {
+        // ---- MMA issuer: the whole warp walks, one lane issues (what the instructions take then stays in uniform registers) ----
+        const bool lead = ptx::elect_one();
         const uint32_t idesc_s = ptx::idesc_bf16_f32_ex(kPtRows, kPtKeys, 0), idesc_o = ptx::idesc_bf16_f32_ex(kPtRows, D, 1);
-        const int steps = D / 16;
+        const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        const int ksteps = D / 16;
         auto product_s = [&](int t, int s) {
             const uint64_t qd = ptx::smem_desc_sw128(base + t * kPtSlot), kd = ptx::smem_desc_sw128(base + kPtSmemK + s * kPtSlot);
+            if (lead) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < steps) {
-                    const uint32_t at = ((i >> 2) * kPtHalf + (i & 3) * 32) >> 4;
-                    ptx::mma_bf16_ss(tmem + t * 128, qd + at, kd + at, idesc_s, i > 0);
-                }
-            ptx::mma_commit(s_full(t));
+                for (int i = 0; i < 8; ++i)
+                    if (i < ksteps) {
+                        const uint32_t at = ((i >> 2) * kPtHalf + (i & 3) * 32) >> 4;
+                        ptx::mma_bf16_ss(tmem_u + t * 128, qd + at, kd + at, idesc_s, i > 0);
+                    }
+                ptx::mma_commit(s_full(t));
+            }
         };
         auto off_lanes = [](int a, int b, int word) -> uint32_t {             // bits of lanes outside [a, b)
             const int lo = max(a - word * 32, 0), hi = min(b - word * 32, 32);
@@ -203,52 +231,80 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             const uint32_t on = (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
             return ~on;
         };
-        PtWalk w(segs, b0), ahead(segs, b0);
-        uint32_t done[2] = {0, 0};
-        bool ok = ptx::mbar_wait(k_full(0), 0, abort_flag);
+        PtWalk w(segs, b0, tt, G);
+        uint32_t done[2][2] = {{0, 0}, {0, 0}};                  // products of the weights of either half, a tile
+        bool ok = ptx::mbar_wait(q_full, 0, abort_flag) && ptx::mbar_wait(k_full(0), 0, abort_flag);
         if (ok) {
             ptx::tc_fence_after_sync();
-            for (int t = 0; t < 2; ++t) if (ahead.active(t, tt, G)) product_s(t, 0);
-            ptx::mma_commit(k_empty(0));
-        }
-        const int n = b1 - b0;
-        for (int j = 0; j < n && ok; ++j, w.next()) {
-            const int s = j & 1;
-            const bool more = j + 1 < n;
-            ahead.next();
-            ok = ptx::mbar_wait(v_full(s), (j >> 1) & 1, abort_flag);
-            for (int t = 0; t < 2 && ok; ++t) {
-                int a, b;
-                w.rows(t, tt, G, a, b);
-                if (a < b) {
-                    ok = ptx::mbar_wait(p_ready(t), done[t] & 1, abort_flag);
-                    if (!ok) break;
-                    ++done[t];
-                    ptx::tc_fence_after_sync();
-                    // (rows beyond the tile's tokens take part in a prefix's products: nobody reads them)
-                    const bool all = a == 0 && (w.seg == 0 && w.s().toks == count);
-                    const uint4 off = all ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(off_lanes(a, b, 0), off_lanes(a, b, 1), off_lanes(a, b, 2), off_lanes(a, b, 3));
-                    const uint64_t vd = ptx::smem_desc_sw128_mn(base + kPtSmemV + s * kPtSlot, kPtHalf);
 #pragma unroll
-                    for (int i = 0; i < kPtKeys / 16; ++i)
-                        ptx::mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + i * 8, vd + ((i * 16 * 128) >> 4), idesc_o, off);
-                }
-                if (more && ahead.active(t, tt, G)) {
-                    ok = ptx::mbar_wait(k_full(s ^ 1), ((j + 1) >> 1) & 1, abort_flag);
-                    if (!ok) break;
-                    ptx::tc_fence_after_sync();
-                    product_s(t, s ^ 1);
-                }
-            }
-            if (!ok) break;
-            ptx::mma_commit(v_empty(s));
-            if (more) ptx::mma_commit(k_empty(s ^ 1));
+            for (int t = 0; t < 2; ++t) if (w.active(t)) product_s(t, 0);
+            if (lead) ptx::mma_commit(k_empty(0));
         }
-        if (ok) { ptx::mma_commit(s_full(0)); ptx::mma_commit(s_full(1)); }       // the last sums are complete
+        for (int j = 0; b0 + j < b1 && ok; ++j) {
+            const int s = j & 1, steps = w.steps();
+            const bool more = b0 + j + 1 < b1;
+            // (rows beyond the tiles' tokens take part in the products of what all rows see: nobody reads them)
+            const bool all = w.seg == 0 && w.s.toks == count;
+            const int ra[2] = {w.ra[0], w.ra[1]}, rb[2] = {w.rb[0], w.rb[1]};
+            if (more) w.next(tt, G);
+            ok = ptx::mbar_wait(v_full(s), (j >> 1) & 1, abort_flag);
+            if (ok && more) ok = ptx::mbar_wait(k_full(s ^ 1), ((j + 1) >> 1) & 1, abort_flag);
+            if (!ok) break;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (ra[t] < rb[t]) {
+                    const uint32_t o = tmem_u + 256 + t * 128;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h >= steps) break;
+                        ok = ok && ptx::mbar_wait(p_ready(t, h), done[t][h] & 1, abort_flag);
+                        if (!ok) break;
+                        ++done[t][h];
+                        ptx::tc_fence_after_sync();
+                        const uint64_t vd = ptx::smem_desc_sw128_mn(base + kPtSmemV + s * kPtSlot + h * 64 * 128, kPtHalf);
+                        const uint32_t pa = tmem_u + t * 128 + h * 32;
+                        if (lead) {
+                            if (all) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) ptx::mma_bf16_ts(o, pa + i * 8, vd + ((i * 16 * 128) >> 4), idesc_o);
+                            } else {
+                                const uint4 off = make_uint4(off_lanes(ra[t], rb[t], 0), off_lanes(ra[t], rb[t], 1), off_lanes(ra[t], rb[t], 2), off_lanes(ra[t], rb[t], 3));
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) ptx::mma_bf16_ts(o, pa + i * 8, vd + ((i * 16 * 128) >> 4), idesc_o, off);
+                            }
+                        }
+                    }
+                    if (!ok) break;
+                }
+                if (more && w.active(t)) product_s(t, s ^ 1);
+            }
+            if (ok && lead) {
+                ptx::mma_commit(v_empty(s));
+                if (more) ptx::mma_commit(k_empty(s ^ 1));
+            }
+        }
+        if (ok && lead) { ptx::mma_commit(s_full(0)); ptx::mma_commit(s_full(1)); }       // the last sums are complete
     } else if (working && warp < 8) {
         // ---- softmax: a row a thread --------------------------------------------------------------------------------
         const int t = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16, tmem_s = tmem + t * 128 + lanes, tmem_o = tmem + 256 + t * 128 + lanes;
+        {
+            // queries into shared memory, 128-byte rows with the 128-byte swizzle, zeros beyond the tile's rows
+            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q);
+            const int chunks = halves * 8, tokens = min(count - t * tt, tt);
+            if (tokens > 0) {
+#pragma unroll 4
+                for (int i = threadIdx.x & 127; i < kPtRows * chunks; i += 128) {
+                    const int qr = i / chunks, c = i % chunks, qt = qr / G;
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (qt < tokens && c * 8 < D)
+                        x = *reinterpret_cast<const uint4*>(q + (size_t)p.toks[tile.first + t * tt + qt] * p.q_stride + (size_t)(kvh * G + qr % G) * D + c * 8);
+                    *reinterpret_cast<uint4*>(smem + t * kPtSlot + (c >> 3) * kPtHalf + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = x;
+                }
+                ptx::fence_proxy_async_shared();
+            }
+            ptx::mbar_arrive(q_full);
+        }
         const int tok = t * tt + r / G;                          // of the block's tokens
         const bool row_valid = r / G < tt && tok < count;
         const int token = row_valid ? p.toks[tile.first + tok] : -1;
@@ -262,17 +318,18 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int c = 0; c < 4; ++c) if (c * 32 < D) ptx::tmem_store_32_nowait(tmem_o + c * 32, zero);
             ptx::tmem_store_wait();
         }
-        PtWalk w(segs, b0);
+        PtWalk w(segs, b0, tt, G);
         uint32_t seen = 0;
         bool ok = true;
-        for (int j = 0; b0 + j < b1 && ok; ++j, w.next()) {
-            int ra, rb;
-            w.rows(t, tt, G, ra, rb);
-            const int key0 = w.key(), end = w.s().key1 - key0;   // block rows beyond `end` belong to nobody
-            const bool shared = w.seg == 0 && w.s().toks == count && (!p.whole || p.group_len[tile.g] > 0);
-            if (end < kPtKeys && (t == 0 ? ra < rb : !w.active(0, tt, G))) {
-                // one tile's threads clear such value rows before the products read them: a weight of zero times what is not
-                // finite would not be zero
+        const float2 rate = make_float2(p.scale_log2, p.scale_log2);
+        for (int j = 0; b0 + j < b1 && ok; ++j, w.next(tt, G)) {
+            const int ra = t == 0 ? w.ra[0] : w.ra[1], rb = t == 0 ? w.rb[0] : w.rb[1];
+            if (ra >= rb) continue;
+            const int end = w.s.key1 - w.key, steps = w.steps();                     // block rows beyond `end` belong to nobody
+            const bool shared = w.seg == 0 && len > 0;
+            if (end < steps * 64) {
+                // such value rows are cleared before the product reads them: a weight of zero times what is not finite would not be
+                // zero (each tile clears them for its own product; the other may be behind)
                 const int s = j & 1;
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(v_full(s), (j >> 1) & 1, abort_flag));
                 if (!ok) break;
@@ -282,52 +339,53 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 ptx::fence_proxy_async_shared();
             }
-            if (ra >= rb) continue;
+            int c0 = 0, c1 = end;                                // columns of the block that this row sees
+            if (!shared) {
+                c0 = w.s.key0 - w.key;
+                c1 = r >= ra && r < rb ? min(end, pos - w.key + 1) : 0;
+            }
+            const bool masks = __any_sync(0xffffffffu, c0 > 0 || c1 < kPtKeys);
+            const bool mine = shared || (rb > quad * 32 && ra < quad * 32 + 32);       // (a warp none of whose rows sees the block has nothing to do)
             ok = __all_sync(0xffffffffu, ptx::mbar_wait(s_full(t), seen & 1, abort_flag));
             if (!ok) break;
-            ++seen;
             ptx::tc_fence_after_sync();
-            if (shared || (rb > quad * 32 && ra < quad * 32 + 32)) {        // (a warp none of whose rows sees the block has nothing to do)
-                float sv[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) ptx::tmem_load_32_nowait(tmem_s + c * 32, sv + c * 32);
+            ++seen;
+            // twice over the row, 64 keys at a time (as straight code with the whole row in registers it spilled and was 2% slower)
+            float2 sum = make_float2(0.f, 0.f), sum2 = make_float2(0.f, 0.f);
+            float2 off = make_float2(0.f, 0.f);
+            auto scores = [&](int h, float* sv) {                // the row's scores of 64 keys, unseen ones taken out
+                ptx::tmem_load_32_nowait(tmem_s + h * 64, sv);
+                ptx::tmem_load_32_nowait(tmem_s + h * 64 + 32, sv + 32);
                 ptx::tmem_load_wait();
-                int c0 = 0, c1 = min(end, kPtKeys);              // columns this row sees
-                if (!shared) {
-                    const bool mine = r >= ra && r < rb;
-                    c0 = max(w.s().key0 - key0, 0);
-                    c1 = mine ? min(c1, pos - key0 + 1) : 0;
-                }
-                if (__any_sync(0xffffffffu, c0 > 0 || c1 < kPtKeys)) {
+                if (masks) {
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) if (c < c0 || c >= c1) sv[c] = -INFINITY;
+                    for (int i = 0; i < 64; ++i) if (h * 64 + i < c0 || h * 64 + i >= c1) sv[i] = -INFINITY;
                 }
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            };
+            if (mine) {
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int h = 0; h < steps; ++h) {
+                    float sv[64];
+                    scores(h, sv);
+                    float m4[4] = {mx, sv[0], sv[1], sv[2]};
 #pragma unroll
-                for (int c = 0; c < 128; c += 2) m4[(c >> 1) & 3] = fmaxf(m4[(c >> 1) & 3], fmaxf(sv[c], sv[c + 1]));
-                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;      // scale > 0
+                    for (int i = 3; i < 59; i += 8) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) m4[q] = fmaxf(fmaxf(m4[q], sv[i + 2 * q]), sv[i + 2 * q + 1]);
+                    }
+                    m4[0] = fmaxf(fmaxf(m4[0], sv[59]), sv[60]); m4[1] = fmaxf(fmaxf(m4[1], sv[61]), sv[62]);
+                    m4[2] = fmaxf(m4[2], sv[63]);
+                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                }
+                mx *= p.scale_log2;                              // scale > 0
                 float corr = 1.f;
                 if (mx > m_ref + 8.f) {
                     corr = m_ref == -INFINITY ? 0.f : ptx::ex2_approx(m_ref - mx);
                     m_ref = mx;
+                    l *= corr;
                 }
-                const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-                float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float e0 = ptx::ex2_approx(fmaf(sv[c * 32 + 2 * i], p.scale_log2, -ref));
-                        const float e1 = ptx::ex2_approx(fmaf(sv[c * 32 + 2 * i + 1], p.scale_log2, -ref));
-                        s4[i & 3] += e0 + e1;
-                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(e0, e1);
-                        pk[i] = *reinterpret_cast<const uint32_t*>(&b2);
-                    }
-                    ptx::tmem_store_16_nowait(tmem_s + c * 16, pk);
-                }
-                l = l * corr + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
-                if (__any_sync(0xffffffffu, corr != 1.f)) {      // rare: rescale these rows of O (P V of the block before is done)
+                if (seen > 1 && __any_sync(0xffffffffu, corr != 1.f)) {              // rare: rescale these rows of O
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         if (c * 32 < D) {
@@ -339,11 +397,37 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                             ptx::tmem_store_32_nowait(tmem_o + c * 32, v);
                         }
                     }
+                    ptx::tmem_store_wait();
                 }
-                ptx::tmem_store_wait();
+                const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+                off = make_float2(-ref, -ref);
             }
-            ptx::tc_fence_before_sync();
-            ptx::mbar_arrive(p_ready(t));
+#pragma unroll 1
+            for (int h = 0; h < steps; ++h) {
+                if (mine) {
+                    float sv[64];
+                    scores(h, sv);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 x = fma_pair(make_float2(sv[u * 32 + 2 * i], sv[u * 32 + 2 * i + 1]), rate, off);
+                            const float2 e = (i & 3) == 3 ? exp2_poly(x) : make_float2(ptx::ex2_approx(x.x), ptx::ex2_approx(x.y));
+                            if (i & 1) sum = add_pair(sum, e); else sum2 = add_pair(sum2, e);
+                            const __nv_bfloat162 b2 = __floats2bfloat162_rn(e.x, e.y);
+                            pk[i] = *reinterpret_cast<const uint32_t*>(&b2);
+                        }
+                        // (over scores that have been read: 16 columns of weights for every 32 of scores)
+                        ptx::tmem_store_16_nowait(tmem_s + h * 32 + u * 16, pk);
+                    }
+                    ptx::tmem_store_wait();
+                }
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(p_ready(t, h));
+            }
+            l += (sum.x + sum.y) + (sum2.x + sum2.y);
         }
         if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(s_full(t), seen & 1, abort_flag));
         if (ok) {
@@ -395,10 +479,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             }
             ptx::tc_fence_before_sync();
         }
-    } else if (!working && found && p.whole && warp < 8) {
+    } else if (!working && warp < 8) {
         // a piece without blocks: empty parts for the merge
         const int t = warp >> 2, r = (warp & 3) * 32 + lane, tok = t * tt + r / G;
-        if (r / G < tt && tok < count) {
+        if (r / G < tt && tok < count && !(base & 1023u)) {
             const size_t at = ((size_t)p.toks[tile.first + tok] * p.n_heads + kvh * G + r % G) * (p.pieces + p.own_splits) + split;
             *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(-INFINITY, 0.f);
         }

@@ -42,16 +42,34 @@ __host__ __device__ __forceinline__ int prefix_pieces_used(int len, int pieces) 
 
 // Tile t of the prefixes' query rows, `tile_tokens` tokens each: which group, which of its tokens.  Groups without a prefix
 // have no tiles (unless their own keys are walked, too).  False: there is no such tile.
-struct PrefixTile { int g, first, count; };          // toks[first .. first + count)
+// (A lane a group, thirty-two at a time: one round of loads finds the tile.)  All lanes of a warp call this together.
+struct PrefixTile { int g, first, count, len; };     // toks[first .. first + count); the group's prefix
 __device__ __forceinline__ bool prefix_tile(const PrefixParams& p, int t, int tile_tokens, PrefixTile& out) {
-    for (int g = 0; g < p.n_groups; ++g) {
-        if (p.group_len[g] <= 0 && !p.whole) continue;
-        const int a = p.tok_first[g], n = p.tok_first[g + 1] - a, tiles = (n + tile_tokens - 1) / tile_tokens;
-        if (t < tiles) {
-            out.g = g; out.first = a + t * tile_tokens; out.count = min(tile_tokens, n - t * tile_tokens);
+    const int lane = threadIdx.x & 31;
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
+        const int g = g0 + lane;
+        int len = 0, a = 0, n = 0, tiles = 0;
+        if (g < p.n_groups) {
+            len = p.group_len[g]; a = p.tok_first[g]; n = p.tok_first[g + 1] - a;
+            tiles = len > 0 || p.whole ? (n + tile_tokens - 1) / tile_tokens : 0;
+        }
+        int last = tiles;                            // tiles up to and with this lane's group
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, last, o);
+            if (lane >= o) last += x;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, last > t);
+        if (behind) {
+            const int at = __ffs(behind) - 1;
+            const int mine = t - (__shfl_sync(0xffffffffu, last, at) - __shfl_sync(0xffffffffu, tiles, at));
+            out.g = g0 + at;
+            out.first = __shfl_sync(0xffffffffu, a, at) + mine * tile_tokens;
+            out.count = min(tile_tokens, __shfl_sync(0xffffffffu, n, at) - mine * tile_tokens);
+            out.len = __shfl_sync(0xffffffffu, len, at);
             return true;
         }
-        t -= tiles;
+        t -= __shfl_sync(0xffffffffu, last, 31);
     }
     return false;
 }

@@ -284,6 +284,12 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Writes 8 consecutive float columns of this thread's TMEM lane; pair with tmem_store_wait().
+__device__ __forceinline__ void tmem_store_8_nowait(uint32_t taddr, const float* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 // Writes 16 consecutive 32-bit columns of this thread's TMEM lane; pair with tmem_store_wait().
 __device__ __forceinline__ void tmem_store_16_nowait(uint32_t taddr, const uint32_t* r) {
     asm volatile(
@@ -291,6 +297,20 @@ __device__ __forceinline__ void tmem_store_16_nowait(uint32_t taddr, const uint3
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+// True in one lane of a warp that is all here.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+// D[tmem] += A[tmem] * B[smem], A in bfloat16 pairs, 8 columns a K step of 16.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc) : "memory");
 }
 // D[tmem] += A[tmem] * B[smem]: A holds bfloat16 pairs, 8 columns a K step of 16.  Lanes whose bit is set in `off` keep what
 // they hold (bit i of off.x: lane i, of off.y: lane 32 + i, ..).
