@@ -33,7 +33,7 @@ prefix_rows_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
     if (prefix) {
         PrefixTile t;
         if (split >= p.pieces || !prefix_tile(p, blockIdx.x, tt, t)) return;
-        const int len = p.group_len[t.g], keys = prefix_piece(len, p.pieces);
+        const int len = p.group_len[t.g], keys = prefix_piece(len, p.pieces, p.unit);
         lo = split * keys; hi = min(len, lo + keys); slot = split; n_tok = t.count; seq = p.group_seq[t.g];
         if (lo >= hi) return;
         if ((int)threadIdx.x < kPrRows) row_token[threadIdx.x] = (int)threadIdx.x / G < n_tok ? p.toks[t.first + threadIdx.x / G] : -1;
@@ -262,7 +262,6 @@ extern "C" int mdma_prefix_attention(const long long* words, int n_words, float 
                  "prefix_attention: heads %d / kv heads %d / head_dim %d is outside its limits (head_dim a multiple of 16 up to 128, group up to 64)",
                  p.n_heads, p.n_kv_heads, p.head_dim);
     MDMA_REQUIRE(p.q_stride % 8 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache) & 15) == 0, "prefix_attention: rows must be 16-byte aligned");
-    MDMA_REQUIRE(((uintptr_t)p.part_o & 15) == 0, "prefix_attention: the scratch must be 16-byte aligned");
     MDMA_REQUIRE(((uintptr_t)p.out & 15) == 0, "prefix_attention: the results must be 16-byte aligned");
     const bool tiled = p.page_size % 64 == 0;
     MDMA_REQUIRE(!p.whole || tiled, "prefix_attention: whole lists of keys want pages of a multiple of 64 tokens");

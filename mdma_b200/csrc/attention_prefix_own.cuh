@@ -181,7 +181,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
     }
     const bool joins = p.own_splits == 1;
-    const int used = joins ? prefix_pieces_used(skip, p.pieces) : 0, slots = p.pieces + p.own_splits;
+    const int used = joins ? prefix_pieces_used(skip, p.pieces, p.unit) : 0, slots = p.pieces + p.own_splits;
     const size_t row0 = (size_t)token * p.n_heads + kvh * G;
     chain_wait();                                                // the prefixes' parts are there, and all that was waited for before them
     __syncthreads();

@@ -1,178 +1,254 @@
 // Attention over shared prefixes on the CUDA cores: the true 32-bit engine's, and bfloat16 of any geometry (head sizes up to
 // 256, any page size).  See prefix.cuh for the parts and how they join.
 //
-// A block takes 32 query rows of one kv head, (token, query head of the group) pairs, and walks its keys in tiles of 32:
-// keys and values staged in shared memory as floats, a thread holds the scores of 2 rows x 4 keys and the sums of 2 rows x
-// head_dim / 8 numbers.  Rows of a prefix tile come from all members of a group, so a key row is read once for 32 rows.
+// A block takes a tile of 8, 32 or 64 query rows of one kv head, (token, query head of the group) pairs, and walks its keys 32
+// at a time: keys and values are staged in shared memory as floats, the next 32 on their way while these are worked on; a
+// thread holds the scores of a few rows x keys and as many rows' sums.  Rows of a prefix tile come from all members of a group,
+// so a key row is read once for all of them; 64 rows make four rows x four keys a thread, which the multiply-add units need to
+// be fed from shared memory; the own keys of a single token are worked on by eight rows of sixteen threads.  The prefixes' kernel
+// and that of the own keys run side by side, a third one joins the parts.
+#include "mma_tiles.cuh"
 #include "prefix.cuh"
 
 namespace mdma {
 
-constexpr int kPsRows = 32, kPsKeys = 32, kPsThreads = 128;
+constexpr int kPsKeys = 32, kPsThreads = 128;
 
-template <typename T, int DC>                        // DC: head_dim rounded up to a multiple of 32, over 32
+// RG groups of threads, RT rows each; the KG = 128 / RG threads of a group hold KT = 32 / KG keys and 4 of every 4 KG numbers of a head.
+template <int RG, int RT, int DC>
+struct PsShape {
+    static constexpr int kRows = RG * RT, kKG = kPsThreads / RG, kKT = kPsKeys / kKG, kPitch = DC * 4 * kKG + 4;
+    static constexpr int kFloats = (kRows + 4 * kPsKeys) * kPitch + kRows * (kPsKeys + 1);
+};
+
+template <typename T, int RG, int RT, int DC>        // DC: steps of 4 KG numbers that cover a head
 __global__ void __launch_bounds__(kPsThreads)
-prefix_simple_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
-    constexpr int kPitch = DC * 32 + 4;              // floats of a staged row
+prefix_simple_kernel(const PrefixParams p, int own_tiles, int wide) {
+    using S = PsShape<RG, RT, DC>;
+    constexpr int kRows = S::kRows, KG = S::kKG, KT = S::kKT, kPitch = S::kPitch, kWidth = DC * 4 * KG;
     extern __shared__ __align__(16) float ps_smem[];
     float* sq = ps_smem;                             // [rows][pitch]
-    float* sk = sq + kPsRows * kPitch;
-    float* sv = sk + kPsKeys * kPitch;
-    float* sp = sv + kPsKeys * kPitch;               // [rows][keys + 1]
-    __shared__ int row_token[kPsRows], row_last[kPsRows];
+    float* skv = sq + kRows * kPitch;                // [stage][keys, values][32][pitch]
+    float* sp = skv + 4 * kPsKeys * kPitch;          // [rows][33]
+    __shared__ int row_token[kRows], row_last[kRows];
 
-    chain_release();
-    chain_wait();
-    const int G = p.group, D = p.head_dim, kvh = blockIdx.y, tt = kPsRows / G > 0 ? kPsRows / G : 1;
-    const bool prefix = (int)blockIdx.x < prefix_tiles;
-    const int heads_at = G > kPsRows ? (int)blockIdx.z % ((G + kPsRows - 1) / kPsRows) * kPsRows : 0;     // first head of the group in this tile
-    const int heads = min(G - heads_at, kPsRows), split = G > kPsRows ? (int)blockIdx.z / ((G + kPsRows - 1) / kPsRows) : blockIdx.z;
+    const int G = p.group, D = p.head_dim, kvh = blockIdx.y, tt = kRows / G > 0 ? kRows / G : 1;
+    const int parts = (G + kRows - 1) / kRows, heads_at = (int)blockIdx.z % parts * kRows;       // first head of the group in this tile
+    const int heads = min(G - heads_at, kRows), split = blockIdx.z / parts;
     int lo, hi, slot, n_tok, seq;
-    if (prefix) {
+    if (own_tiles == 0) {                            // prefixes
+        chain_wait();
+        chain_release();                             // (only now: the own keys' kernel counts on what this one waited for)
         PrefixTile t;
-        if (split >= p.pieces || !prefix_tile(p, blockIdx.x, tt, t)) return;
-        const int len = p.group_len[t.g], keys = prefix_piece(len, p.pieces);
-        lo = split * keys; hi = min(len, lo + keys); slot = split; n_tok = t.count; seq = p.group_seq[t.g];
+        if (!prefix_tile(p, blockIdx.x, tt, t)) return;
+        const int keys = prefix_piece(t.len, p.pieces, p.unit);
+        lo = split * keys; hi = min(t.len, lo + keys); slot = split; n_tok = t.count; seq = p.group_seq[t.g];
         if (lo >= hi) return;
-        if ((int)threadIdx.x < kPsRows) {
-            const int r = threadIdx.x;
+        for (int r = threadIdx.x; r < kRows; r += kPsThreads) {
             row_token[r] = r / heads < n_tok ? p.toks[t.first + r / heads] : -1;
             row_last[r] = hi - 1;
         }
     } else {
-        seq = ((int)blockIdx.x - prefix_tiles) / own_tiles;
-        const int tok0 = ((int)blockIdx.x - prefix_tiles) % own_tiles * tt, n_new = p.seq_start[seq + 1] - p.seq_start[seq];
-        if (split >= p.own_splits || tok0 >= n_new) return;
+        chain_release();
+        seq = (int)blockIdx.x / own_tiles;
+        const int tok0 = (int)blockIdx.x % own_tiles * tt, n_new = p.seq_start[seq + 1] - p.seq_start[seq];
+        if (tok0 >= n_new) { chain_wait(); return; }
         n_tok = min(tt, n_new - tok0);
         const int skip = p.seq_skip[seq], end = p.seq_pos0[seq] + tok0 + n_tok;
         const int keys = ((end - skip + p.own_splits - 1) / p.own_splits + kPsKeys - 1) / kPsKeys * kPsKeys;
         lo = skip + split * keys; hi = min(end, lo + keys); slot = p.pieces + split;
-        if ((int)threadIdx.x < kPsRows) {
-            const int r = threadIdx.x;
+        for (int r = threadIdx.x; r < kRows; r += kPsThreads) {
             row_token[r] = r / heads < n_tok ? p.seq_start[seq] + tok0 + r / heads : -1;
             row_last[r] = p.seq_pos0[seq] + tok0 + min(r / heads, n_tok - 1);
         }
     }
-    __syncthreads();
-    const T* q = reinterpret_cast<const T*>(p.q);
-    for (int i = threadIdx.x; i < kPsRows * kPitch; i += kPsThreads) {
-        const int r = i / kPitch, d = i % kPitch, token = row_token[r];
-        sq[i] = token >= 0 && d < D ? to_float(q[token * p.q_stride + (long)(kvh * G + heads_at + r % heads) * D + d]) * p.scale_log2 : 0.f;
-    }
     const int* pages = p.page_table + (size_t)p.seq_slot[seq] * p.max_pages;
     const T* kc = reinterpret_cast<const T*>(p.k_cache);
     const T* vc = reinterpret_cast<const T*>(p.v_cache);
-    const int ty = threadIdx.x >> 3, tx = threadIdx.x & 7, r0 = ty * 2;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[2][DC][4];
+    auto load = [&](int key0, int stage) {
+        float* dk = skv + stage * 2 * kPsKeys * kPitch;
+        float* dv = dk + kPsKeys * kPitch;
+        if (wide) {                                  // floats, 16 bytes at a time, asynchronously
+            const int chunks = kWidth / 4;
+#pragma unroll 4
+            for (int i = threadIdx.x; i < kPsKeys * chunks; i += kPsThreads) {
+                const int r = i / chunks, c = i % chunks, key = key0 + r;
+                const bool valid = key < hi && c * 4 < D;          // rows beyond belong to nobody: zeros instead
+                size_t at = 0;
+                if (valid) at = (((size_t)pages[key / p.page_size] * p.page_size + key % p.page_size) * p.n_kv_heads + kvh) * D + c * 4;
+                cp_async_16((uint32_t)__cvta_generic_to_shared(dk + r * kPitch + c * 4), kc + at, valid);
+                cp_async_16((uint32_t)__cvta_generic_to_shared(dv + r * kPitch + c * 4), vc + at, valid);
+            }
+        } else {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < kPsKeys * kWidth; i += kPsThreads) {
+                const int r = i / kWidth, d = i % kWidth, key = key0 + r;
+                float k = 0.f, v = 0.f;
+                if (key < hi && d < D) {
+                    const size_t at = (((size_t)pages[key / p.page_size] * p.page_size + key % p.page_size) * p.n_kv_heads + kvh) * D + d;
+                    k = to_float(kc[at]); v = to_float(vc[at]);
+                }
+                dk[r * kPitch + d] = k; dv[r * kPitch + d] = v;
+            }
+        }
+        cp_async_commit();
+    };
+    if (lo < hi) load(lo, 0);
+    __syncthreads();                                 // the rows' tokens are known
+    const T* q = reinterpret_cast<const T*>(p.q);
+    if (wide) {
+        constexpr int chunks = kWidth / 4;
+#pragma unroll 8
+        for (int i = threadIdx.x; i < kRows * chunks; i += kPsThreads) {
+            const int r = i / chunks, c = i % chunks, token = row_token[r];
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (token >= 0 && c * 4 < D) x = *reinterpret_cast<const float4*>(q + token * p.q_stride + (long)(kvh * G + heads_at + r % heads) * D + c * 4);
+            *reinterpret_cast<float4*>(sq + r * kPitch + c * 4) = make_float4(x.x * p.scale_log2, x.y * p.scale_log2, x.z * p.scale_log2, x.w * p.scale_log2);
+        }
+    } else
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kRows * kWidth; i += kPsThreads) {
+        const int r = i / kWidth, d = i % kWidth, token = row_token[r];
+        sq[r * kPitch + d] = token >= 0 && d < D ? to_float(q[token * p.q_stride + (long)(kvh * G + heads_at + r % heads) * D + d]) * p.scale_log2 : 0.f;
+    }
+    const int ty = threadIdx.x / KG, tx = threadIdx.x % KG, r0 = ty * RT;
+    float m[RT], l[RT], acc[RT][DC][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < RT; ++i) {
+        m[i] = -INFINITY; l[i] = 0.f;
 #pragma unroll
         for (int c = 0; c < DC; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
-    const bool working = r0 < n_tok * heads;         // (whole groups of eight lanes)
-    for (int key0 = lo; key0 < hi; key0 += kPsKeys) {
+    }
+    const bool working = r0 < n_tok * heads;         // (whole groups of threads)
+    const uint32_t group = ((1u << KG) - 1u) << ((threadIdx.x & 31) / KG * KG);      // this group's lanes
+    int stage = 0;
+    for (int key0 = lo; key0 < hi; key0 += kPsKeys, stage ^= 1) {
+        if (key0 + kPsKeys < hi) load(key0 + kPsKeys, stage ^ 1); else cp_async_commit();
+        cp_async_wait<1>();
         __syncthreads();
-        for (int i = threadIdx.x; i < kPsKeys * DC * 32; i += kPsThreads) {
-            const int r = i / (DC * 32), d = i % (DC * 32), key = key0 + r;
-            float k = 0.f, v = 0.f;                  // rows beyond the last key belong to nobody: never read
-            if (key < hi && d < D) {
-                const size_t at = (((size_t)pages[key / p.page_size] * p.page_size + key % p.page_size) * p.n_kv_heads + kvh) * D + d;
-                k = to_float(kc[at]); v = to_float(vc[at]);
-            }
-            sk[r * kPitch + d] = k; sv[r * kPitch + d] = v;
-        }
-        __syncthreads();
-        float s[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        const float* sk = skv + stage * 2 * kPsKeys * kPitch;
+        const float* sv = sk + kPsKeys * kPitch;
         if (working) {
-#pragma unroll 4
-            for (int d = 0; d < DC * 32; d += 4) {
-                const float4 a = *reinterpret_cast<const float4*>(sq + r0 * kPitch + d), b = *reinterpret_cast<const float4*>(sq + (r0 + 1) * kPitch + d);
+            float s[RT][KT];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float4 k = *reinterpret_cast<const float4*>(sk + (tx + 8 * j) * kPitch + d);
-                    s[0][j] = fmaf(a.x, k.x, fmaf(a.y, k.y, fmaf(a.z, k.z, fmaf(a.w, k.w, s[0][j]))));
-                    s[1][j] = fmaf(b.x, k.x, fmaf(b.y, k.y, fmaf(b.z, k.z, fmaf(b.w, k.w, s[1][j]))));
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < KT; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < kWidth; d += 4) {
+                float4 a[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) a[i] = *reinterpret_cast<const float4*>(sq + (r0 + i) * kPitch + d);
+#pragma unroll
+                for (int j = 0; j < KT; ++j) {
+                    const float4 k = *reinterpret_cast<const float4*>(sk + (tx + KG * j) * kPitch + d);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) s[i][j] = fmaf(a[i].x, k.x, fmaf(a[i].y, k.y, fmaf(a[i].z, k.z, fmaf(a[i].w, k.w, s[i][j]))));
                 }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int last = min(row_last[r0 + i], hi - 1);
-            float mx = m[i];
+            for (int i = 0; i < RT; ++i) {
+                const int last = min(row_last[r0 + i], hi - 1);
+                float mx = m[i];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (key0 + tx + 8 * j > last) s[i][j] = -INFINITY;
-                mx = fmaxf(mx, s[i][j]);
+                for (int j = 0; j < KT; ++j) {
+                    if (key0 + tx + KG * j > last) s[i][j] = -INFINITY;
+                    mx = fmaxf(mx, s[i][j]);
+                }
+#pragma unroll
+                for (int o = 1; o < KG; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(group, mx, o));
+                const float ref = mx == -INFINITY ? 0.f : mx, corr = exp2f(m[i] - ref);
+                m[i] = mx;
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < KT; ++j) {
+                    const float e = exp2f(s[i][j] - ref);
+                    sum += e;
+                    sp[(r0 + i) * (kPsKeys + 1) + tx + KG * j] = e;
+                }
+                l[i] = l[i] * corr + sum;
+#pragma unroll
+                for (int c = 0; c < DC; ++c) { acc[i][c][0] *= corr; acc[i][c][1] *= corr; acc[i][c][2] *= corr; acc[i][c][3] *= corr; }
             }
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float ref = mx == -INFINITY ? 0.f : mx, corr = exp2f(m[i] - ref);
-            m[i] = mx;
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float e = exp2f(s[i][j] - ref);
-                sum += e;
-                sp[(r0 + i) * (kPsKeys + 1) + tx + 8 * j] = e;
-            }
-            l[i] = l[i] * corr + sum;
-#pragma unroll
-            for (int c = 0; c < DC; ++c) { acc[i][c][0] *= corr; acc[i][c][1] *= corr; acc[i][c][2] *= corr; acc[i][c][3] *= corr; }
         }
-        __syncwarp();                                // a row's weights are written and read by eight lanes of one warp
+        __syncwarp();                                // a row's weights are written and read by threads of one warp
         if (working) {
 #pragma unroll 2
             for (int j = 0; j < kPsKeys; ++j) {
-                const float e0 = sp[r0 * (kPsKeys + 1) + j], e1 = sp[(r0 + 1) * (kPsKeys + 1) + j];
+                float e[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) e[i] = sp[(r0 + i) * (kPsKeys + 1) + j];
 #pragma unroll
                 for (int c = 0; c < DC; ++c) {
-                    const float4 v = *reinterpret_cast<const float4*>(sv + j * kPitch + c * 32 + tx * 4);
-                    acc[0][c][0] = fmaf(e0, v.x, acc[0][c][0]); acc[0][c][1] = fmaf(e0, v.y, acc[0][c][1]);
-                    acc[0][c][2] = fmaf(e0, v.z, acc[0][c][2]); acc[0][c][3] = fmaf(e0, v.w, acc[0][c][3]);
-                    acc[1][c][0] = fmaf(e1, v.x, acc[1][c][0]); acc[1][c][1] = fmaf(e1, v.y, acc[1][c][1]);
-                    acc[1][c][2] = fmaf(e1, v.z, acc[1][c][2]); acc[1][c][3] = fmaf(e1, v.w, acc[1][c][3]);
+                    const float4 v = *reinterpret_cast<const float4*>(sv + j * kPitch + c * 4 * KG + tx * 4);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) {
+                        acc[i][c][0] = fmaf(e[i], v.x, acc[i][c][0]); acc[i][c][1] = fmaf(e[i], v.y, acc[i][c][1]);
+                        acc[i][c][2] = fmaf(e[i], v.z, acc[i][c][2]); acc[i][c][3] = fmaf(e[i], v.w, acc[i][c][3]);
+                    }
                 }
             }
         }
-        __syncwarp();
+        __syncthreads();                             // the stage may be overwritten
     }
+    cp_async_wait<0>();
     const int slots = p.pieces + p.own_splits;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < RT; ++i) {
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+        for (int o = 1; o < KG; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
         const int r = r0 + i;
         if (r >= n_tok * heads) continue;
         const size_t row = (size_t)row_token[r] * p.n_heads + kvh * G + heads_at + r % heads;
         float* to = p.part_o + (row * slots + slot) * D;
 #pragma unroll
-        for (int c = 0; c < DC; ++c)
+        for (int c = 0; c < DC; ++c) {
+            const int d = c * 4 * KG + tx * 4;
+            if (wide) {
+                if (d < D) *reinterpret_cast<float4*>(to + d) = make_float4(acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c * 32 + tx * 4 + e < D) to[c * 32 + tx * 4 + e] = acc[i][c][e];
+                for (int e = 0; e < 4; ++e) if (d + e < D) to[d + e] = acc[i][c][e];
+            }
+        }
         if (tx == 0) { p.part_ml[(row * slots + slot) * 2] = m[i]; p.part_ml[(row * slots + slot) * 2 + 1] = l[i]; }
     }
+    if (own_tiles > 0) chain_wait();                 // whoever waits for this kernel has waited for the prefixes', too
+}
+
+template <typename T, int RG, int RT, int DC>
+static int launch_prefix_simple_as(const PrefixParams& p, bool own, int wide, cudaStream_t stream) {
+    using S = PsShape<RG, RT, DC>;
+    const int G = p.group, tt = S::kRows / G > 0 ? S::kRows / G : 1, parts = (G + S::kRows - 1) / S::kRows;
+    const int own_tiles = own ? (p.max_new + tt - 1) / tt : 0;
+    const long tiles = own ? (long)own_tiles * p.n_seqs : prefix_tiles_bound(p, tt);
+    const int splits = own ? p.own_splits : p.pieces;
+    MDMA_REQUIRE(tiles <= 0x7fffffffl && p.n_kv_heads <= 65535 && splits * parts <= 65535, "prefix_attention: grid too large");
+    auto kernel = prefix_simple_kernel<T, RG, RT, DC>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kFloats * 4);
+    if (e == cudaSuccess) e = launch_chained(kernel, dim3((unsigned)tiles, p.n_kv_heads, splits * parts), dim3(kPsThreads), S::kFloats * 4, stream, p, own_tiles, wide);
+    if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
+    return 0;
+}
+// `rows`: how many of them a block should take
+template <typename T>
+static int launch_prefix_simple_rows(const PrefixParams& p, bool own, int rows, int wide, cudaStream_t stream) {
+    const int D = p.head_dim;
+    if (rows <= 8)
+        return D <= 64 ? launch_prefix_simple_as<T, 8, 1, 1>(p, own, wide, stream) : D <= 128 ? launch_prefix_simple_as<T, 8, 1, 2>(p, own, wide, stream)
+                                                                                           : launch_prefix_simple_as<T, 8, 1, 4>(p, own, wide, stream);
+    if (rows <= 32 || D > 128)
+        return D <= 64 ? launch_prefix_simple_as<T, 16, 2, 2>(p, own, wide, stream) : D <= 128 ? launch_prefix_simple_as<T, 16, 2, 4>(p, own, wide, stream)
+                                                                                           : launch_prefix_simple_as<T, 16, 2, 8>(p, own, wide, stream);
+    return D <= 64 ? launch_prefix_simple_as<T, 16, 4, 2>(p, own, wide, stream) : launch_prefix_simple_as<T, 16, 4, 4>(p, own, wide, stream);
 }
 
 template <typename T>
-static int launch_prefix_simple(const PrefixParams& p, cudaStream_t stream) {
-    const int G = p.group, tt = kPsRows / G > 0 ? kPsRows / G : 1, parts = (G + kPsRows - 1) / kPsRows;
-    const int own_tiles = (p.max_new + tt - 1) / tt;
-    const long prefix_tiles = prefix_tiles_bound(p, tt), tiles = prefix_tiles + (long)own_tiles * p.n_seqs;
-    const int splits = p.pieces > p.own_splits ? p.pieces : p.own_splits;
-    MDMA_REQUIRE(tiles <= 0x7fffffffl && p.n_kv_heads <= 65535 && splits * parts <= 65535, "prefix_attention: grid too large");
-    const dim3 grid((unsigned)tiles, p.n_kv_heads, splits * parts);
-    const int dc = (p.head_dim + 31) / 32;
-    auto run = [&](auto kernel, int pitch_dc) -> int {
-        const int pitch = pitch_dc * 32 + 4, bytes = ((kPsRows + 2 * kPsKeys) * pitch + kPsRows * (kPsKeys + 1)) * 4;
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) e = launch_chained(kernel, grid, dim3(kPsThreads), bytes, stream, p, (int)prefix_tiles, own_tiles);
-        if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
-        return 0;
-    };
-    const int rc = dc <= 2 ? run(prefix_simple_kernel<T, 2>, 2) : dc <= 4 ? run(prefix_simple_kernel<T, 4>, 4) : run(prefix_simple_kernel<T, 8>, 8);
-    if (rc) return rc;
+static int launch_prefix_simple(const PrefixParams& p, int prefix_rows, int own_rows, cudaStream_t stream) {
+    const int wide = sizeof(T) == 4 && p.head_dim % 4 == 0 && p.q_stride % 4 == 0 &&
+                     (((uintptr_t)p.k_cache | (uintptr_t)p.v_cache | (uintptr_t)p.q | (uintptr_t)p.part_o) & 15) == 0;
+    if (int rc = launch_prefix_simple_rows<T>(p, false, prefix_rows, wide, stream)) return rc;
+    if (int rc = launch_prefix_simple_rows<T>(p, true, own_rows, wide, stream)) return rc;
     const long rows = (long)p.n_tokens * p.n_heads;
     const cudaError_t e = launch_chained(prefix_merge_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, p);
     if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
@@ -183,10 +259,13 @@ static int launch_prefix_simple(const PrefixParams& p, cudaStream_t stream) {
 
 using namespace mdma;
 
-extern "C" int mdma_prefix_attention_simple(const long long* words, int n_words, float scale, int dtype, cudaStream_t stream) {
+extern "C" int mdma_prefix_attention_simple(const long long* words, int n_words, float scale, int dtype, int prefix_rows, int own_rows,
+                                            cudaStream_t stream) {
     PrefixParams p;
     if (int rc = prefix_params(words, n_words, scale, &p)) return rc;
+    p.unit = kPsKeys;
+    MDMA_REQUIRE(!p.whole, "prefix_attention: whole lists of keys are the tensor-core kernel's");
     if (p.n_tokens == 0 || p.n_seqs == 0) return 0;
-    MDMA_DISPATCH_DTYPE(dtype, T, return launch_prefix_simple<T>(p, stream));
+    MDMA_DISPATCH_DTYPE(dtype, T, return launch_prefix_simple<T>(p, prefix_rows, own_rows, stream));
     return 0;
 }

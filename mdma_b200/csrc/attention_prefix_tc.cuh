@@ -120,7 +120,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const int count = tile.count, len = tile.len;                // tokens of both tiles; the prefix
     int b0 = 0, b1 = 0;                                          // this block's part of the list
     if (!p.whole) {
-        const int keys = prefix_piece(len, p.pieces), lo = split * keys, hi = min(len, lo + keys);
+        const int keys = prefix_piece(len, p.pieces, p.unit), lo = split * keys, hi = min(len, lo + keys);
         if (lo >= hi) return;
         if (threadIdx.x == 0) {
             segs[0] = {p.group_seq[tile.g], lo, hi, 0, count, 0};

@@ -31,7 +31,7 @@ LIBRARIES = {
              "linear_attention.cu", "chunk_scan.cu", "group_norm.cu", "rotary_latent.cu", "attention_talking.cu",
              "delta_rule.cu", "delta_chunk.cu", "attention_mixed_weights.cu", "attention_finish.cu", "matrix_memory.cu", "cache_pages.cu",
              "attention_prefix_simple.cu"],
-             ["common.cuh", "ptx.cuh", "delta_rule.cuh", "float4.cuh", "rows_product.cuh", "linear_input.cuh", "prefix.cuh"], []),
+             ["common.cuh", "ptx.cuh", "delta_rule.cuh", "float4.cuh", "rows_product.cuh", "linear_input.cuh", "prefix.cuh", "mma_tiles.cuh"], []),
     "tensor": (["gemm_tcgen05.cu", "attention_mma.cu", "attention_tc.cu", "attention_talking_mma.cu",
                 "attention_mixed_weights_mma.cu", "attention_prefix.cu"],
                ["common.cuh", "ptx.cuh", "attention_mma.cuh", "mma_tiles.cuh", "prefix.cuh",

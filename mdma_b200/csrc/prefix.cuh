@@ -23,20 +23,21 @@ struct PrefixParams {
     int n_groups, n_seqs, n_tokens, max_new;
     int n_heads, n_kv_heads, head_dim, group;
     int pieces, own_splits;                          // a prefix in `pieces` pieces at most, own keys in `own_splits`: slots of the parts
+    int unit;                                        // a piece of a prefix is a multiple of so many keys
     int whole;                                       // own_splits 0: all keys of a row tile, prefix and own ones, are one list in `pieces` pieces
     float scale_log2;                                // scale * log2(e)
     const float* sinks; float sink_rate;             // sinks[head] * sink_rate is in powers of two; null: none
     int* status;
 };
 
-// Keys of a piece of a prefix of `len` tokens: a multiple of 128 that follows from the prefix alone, so that a sequence's sums
+// Keys of a piece of a prefix of `len` tokens: a multiple of `unit` that follows from the prefix alone, so that a sequence's sums
 // are cut at the same places whoever shares the step.
-__host__ __device__ __forceinline__ int prefix_piece(int len, int pieces) {
-    return ((len + pieces - 1) / pieces + 127) / 128 * 128;
+__host__ __device__ __forceinline__ int prefix_piece(int len, int pieces, int unit) {
+    return ((len + pieces - 1) / pieces + unit - 1) / unit * unit;
 }
-__host__ __device__ __forceinline__ int prefix_pieces_used(int len, int pieces) {
+__host__ __device__ __forceinline__ int prefix_pieces_used(int len, int pieces, int unit) {
     if (len <= 0) return 0;
-    const int keys = prefix_piece(len, pieces);
+    const int keys = prefix_piece(len, pieces, unit);
     return (len + keys - 1) / keys;
 }
 
@@ -78,7 +79,8 @@ static inline long prefix_tiles_bound(const PrefixParams& p, int tile_tokens) {
     return (long)p.n_tokens / tile_tokens + p.n_groups;
 }
 
-// out[token, head] from its parts: those of its prefix in order, then those of its own keys.  One warp a row.
+// out[token, head] from its parts: those of its prefix in order, then those of its own keys.  One warp a row: a lane a part for the
+// maxima, the sums and the shares (at most 64 parts), then all lanes over the parts' numbers, eight parts in flight.
 template <typename T>
 __global__ void __launch_bounds__(128)
 prefix_merge_kernel(const PrefixParams p) {
@@ -88,29 +90,44 @@ prefix_merge_kernel(const PrefixParams p) {
     const int lane = threadIdx.x & 31;
     if (row >= (long)p.n_tokens * p.n_heads) return;
     const int slots = p.pieces + p.own_splits, D = p.head_dim;
-    const int used = p.whole ? p.pieces : prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces);
-    const float* ml = p.part_ml + row * slots * 2;
-    float m = -INFINITY;
-    for (int s = 0; s < used + p.own_splits; ++s) m = fmaxf(m, ml[2 * (s < used ? s : p.pieces + s - used)]);
-    const float sink = p.sinks ? p.sinks[row % p.n_heads] * p.sink_rate : -INFINITY;
-    float l = 0.f;
-    float acc[8];
+    const int used = p.whole ? p.pieces : prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces, p.unit), parts = used + p.own_splits;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * slots;
+    auto slot_of = [&](int s) { return s < used ? s : p.pieces + s - used; };
+    float2 mine[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int s = 0; s < used + p.own_splits; ++s) {
-        const int slot = s < used ? s : p.pieces + s - used;
-        const float ms = ml[2 * slot];
-        if (ms == -INFINITY) continue;
-        const float f = exp2f(ms - m);
-        l += f * ml[2 * slot + 1];
-        const float* o = p.part_o + (row * slots + slot) * D;
+    for (int u = 0; u < 2; ++u) mine[u] = u * 32 + lane < parts ? ml[slot_of(u * 32 + lane)] : make_float2(-INFINITY, 0.f);
+    const float m = warp_max(fmaxf(mine[0].x, mine[1].x));
+    float share[2], l = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (lane + 32 * j < D) acc[j] = fmaf(f, o[lane + 32 * j], acc[j]);
+    for (int u = 0; u < 2; ++u) {
+        share[u] = mine[u].x == -INFINITY ? -1.f : exp2f(mine[u].x - m);              // a part without keys has no share
+        if (share[u] >= 0.f) l += share[u] * mine[u].y;
     }
-    if (p.sinks) l += exp2f(sink - m);
+    l = warp_sum(l);
+    if (p.sinks) l += exp2f(p.sinks[row % p.n_heads] * p.sink_rate - m);
+    const float* o = p.part_o + row * slots * D;
     T* to = reinterpret_cast<T*>(p.out) + row * D;
+    for (int d0 = 0; d0 < D; d0 += 64) {             // two numbers a lane, 32 apart
+        const int d = d0 + lane;
+        const bool one = d < D, two = d + 32 < D;
+        float a0 = 0.f, a1 = 0.f;
+        for (int s0 = 0; s0 < parts; s0 += 8) {
+            float x0[8], x1[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) if (lane + 32 * j < D) to[lane + 32 * j] = from_float<T>(acc[j] / l);
+            for (int u = 0; u < 8; ++u) {
+                const float* from = o + (size_t)slot_of(min(s0 + u, parts - 1)) * D + d;
+                x0[u] = one ? __ldcg(from) : 0.f; x1[u] = two ? __ldcg(from + 32) : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int s = s0 + u;
+                const float f = __shfl_sync(0xffffffffu, s < 32 ? share[0] : share[1], s & 31);
+                if (s < parts && f >= 0.f) { a0 = fmaf(f, x0[u], a0); a1 = fmaf(f, x1[u], a1); }
+            }
+        }
+        if (one) to[d] = from_float<T>(a0 / l);
+        if (two) to[d + 32] = from_float<T>(a1 / l);
+    }
 }
 
 // The arguments as one array of 64-bit words, in the order below (a step makes this call once a layer: converting thirty
@@ -141,12 +158,15 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     MDMA_REQUIRE(p.head_dim > 0 && p.head_dim <= 256, "prefix_attention: head_dim %d is beyond the limit of 256", p.head_dim);
     MDMA_REQUIRE(p.page_table && p.page_size > 0 && p.max_pages > 0, "prefix_attention: bad cache geometry");
     MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 1 && p.own_splits >= 0, "prefix_attention: bad sizes");
+    MDMA_REQUIRE(p.pieces <= 32 && p.own_splits <= 32, "prefix_attention: %d and %d pieces are beyond the limit of 32", p.pieces, p.own_splits);
     MDMA_REQUIRE(scale > 0.f, "prefix_attention: the score scale must be positive");
     p.group = p.n_heads / p.n_kv_heads;
-    p.whole = p.own_splits == 0;
-    const long long slots = p.whole && p.pieces == 1 ? 0 : (long long)p.n_tokens * p.n_heads * (p.pieces + p.own_splits), need = slots * (p.head_dim + 2);
+    p.whole = p.own_splits == 0; p.unit = 128;
+    const long long slots = p.whole && p.pieces == 1 ? 0 : (long long)p.n_tokens * p.n_heads * (p.pieces + p.own_splits), need = slots ? slots * (p.head_dim + 2) + 4 : 0;
     MDMA_REQUIRE(need == 0 || (scratch && floats >= need), "prefix_attention: %lld floats of scratch are needed, %lld given", need, floats);
-    p.part_o = scratch; p.part_ml = scratch + slots * p.head_dim;
+    MDMA_REQUIRE(((uintptr_t)scratch & 15) == 0, "prefix_attention: the scratch must be 16-byte aligned");
+    // pairs first, so that they lie at multiples of 8 bytes and the sums behind them of 16, whatever the head size
+    p.part_ml = scratch; p.part_o = scratch + (slots * 2 + 3) / 4 * 4;
     return 0;
 }
 

@@ -149,7 +149,7 @@ def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_cont
             parts = sum(ops.prefix_plan(ctx, most, heads, kv_heads))
             if dtype == torch.bfloat16 and ops_tensor.attention_supported(heads, kv_heads, head_dim):
                 parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, sms, page_size)))
-            need = max(need, max_slots * heads * parts * (head_dim + 2))
+            need = max(need, ops.prefix_scratch_floats(max_slots, heads, parts, head_dim))
     return need
 
 

@@ -1168,12 +1168,28 @@ def prefix_split(tile_rows: int, blocks_wanted: int, tokens: int, seqs: int, max
     return pieces, max(1, min(blocks_wanted // own, 32, -(-most_own // 128)))
 
 
-def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int) -> tuple[int, int]:
-    """`prefix_split` for a step on the CUDA cores.  Of single tokens it follows from the most sequences the engine can hold,
-    not from the live ones, so that a request's sums are cut at the same places when a batch mate ends."""
-    one = ctx.max_new == 1
+def _prefix_rows(rows: int) -> int:
+    return 8 if rows <= 8 else 32 if rows <= 32 else 64
+
+
+def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int = 148) -> tuple[int, int]:
+    """(pieces of a prefix, pieces of a sequence's own keys) of a step on the CUDA cores, 32 keys each at least, for about four
+    blocks an SM.  Of single tokens it follows from the most sequences the engine can hold, not from the live ones, so that a
+    request's sums are cut at the same places when a batch mate ends."""
+    one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
-    return prefix_split(32, 4 * 148, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
+    tokens = seqs if one else ctx.n_tokens
+
+    def tiles(rows, of_tokens):                      # blocks of `rows` query rows over so many tokens, all kv heads
+        return -(-of_tokens // max(1, rows // group)) * -(-group // rows) * n_kv_heads
+    pieces = 4 * sms // tiles(_prefix_rows(tokens * group), tokens)
+    own = 4 * sms // (tiles(_prefix_rows(ctx.max_new * group), ctx.max_new) * seqs)
+    return max(1, min(pieces, 32, -(-g.most_len // 32))), max(1, min(own, 32, -(-g.most_own // 32)))
+
+
+def prefix_scratch_floats(tokens: int, n_heads: int, parts: int, head_dim: int) -> int:
+    """Floats of scratch for the parts of so many tokens' softmaxes."""
+    return tokens * n_heads * parts * (head_dim + 2) + 4
 
 
 def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, pieces: int, own_splits: int, scratch, sinks, status,
@@ -1226,10 +1242,12 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
         return
     g = ctx.prefix
     pieces, own = prefix_plan(ctx, g, n_heads, n_kv_heads)
-    need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2)
+    need = prefix_scratch_floats(ctx.n_tokens, n_heads, pieces + own, head_dim)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.float32, device=q.device)
     elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need:
         raise KernelError(f"prefix attention needs {need} floats of scratch, {scratch.numel()} given")
     words = prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sinks, None, False)
-    _call("core", "mdma_prefix_attention_simple", words, _i(32), _f(scale), _i(dtype_code(q.dtype)), _stream(), launches=2)
+    group = n_heads // n_kv_heads
+    _call("core", "mdma_prefix_attention_simple", words, _i(32), _f(scale), _i(dtype_code(q.dtype)),
+          _i(_prefix_rows(ctx.n_tokens * group)), _i(_prefix_rows(ctx.max_new * group)), _stream(), launches=3)

@@ -682,7 +682,7 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     flush_pending(q.device, st)
     g = ctx.prefix
     pieces, own = prefix_plan(ctx, g, n_heads, n_kv_heads, st.sms, view.page_size)
-    need = ctx.n_tokens * n_heads * (pieces + own) * (head_dim + 2) if pieces + own > 1 else 0
+    need = ops.prefix_scratch_floats(ctx.n_tokens, n_heads, pieces + own, head_dim) if pieces + own > 1 else 0
     if own_st is not None:
         st.need(need, "attention over shared prefixes")
         scratch = st.scratch

@@ -283,7 +283,7 @@ class Attention(Part):
             scratch = self.rt.tc.scratch if self.rt.tc is not None and not self.rt.tc.growable else None
         else:
             parts, scratch = sum(ops.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads)), self.rt.prefix_scratch
-        return scratch is None or ctx.n_tokens * self.n_heads * parts * (self.head_dim + 2) <= scratch.numel()
+        return scratch is None or ops.prefix_scratch_floats(ctx.n_tokens, self.n_heads, parts, self.head_dim) <= scratch.numel()
 
     def _attend_shared(self, ctx, row, view, out, sinks=None, sinks_log2=None):
         sizes = (self.n_heads, self.n_kv_heads, self.head_dim, self.scale)
