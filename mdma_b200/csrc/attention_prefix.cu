@@ -213,30 +213,33 @@ static int prefix_cache_map(CUtensorMap* out, const void* cache, const PrefixPar
     return 0;
 }
 
-static bool prefix_own_fits(const PrefixParams& p) {
+static bool prefix_stream_fits(const PrefixParams& p) {
     return p.max_new == 1 && p.group <= 16 && p.page_size % 32 == 0 && p.pieces <= kPoMaxPieces && p.own_splits >= 1;
 }
-static int launch_prefix_own(const PrefixParams& p, int sms, cudaStream_t stream) {
+// The sequences' own keys, or the prefixes.
+template <bool SHARED>
+static int launch_prefix_stream(const PrefixParams& p, int sms, cudaStream_t stream) {
     const int kb = p.head_dim <= 64 && p.page_size % 64 == 0 ? 64 : 32;       // a tile of 8 KB either way
-    const long blocks = (long)p.n_kv_heads * p.own_splits * p.n_seqs;
-    MDMA_REQUIRE(p.n_seqs <= 65535 && blocks <= 0x7fffffffl, "prefix_attention: grid too large");
+    const long items = SHARED ? prefix_tiles_bound(p, 16 / p.group) : p.n_seqs, splits = SHARED ? p.pieces : p.own_splits;
+    const long blocks = p.n_kv_heads * splits * (SHARED ? (p.n_tokens * p.group + 15) / 16 : items);       // (those that have something to do, about)
+    MDMA_REQUIRE(items <= 65535 && p.n_kv_heads * splits <= 0x7fffffffl, "prefix_attention: grid too large");
     CUtensorMap mk, mv;
     if (int rc = prefix_cache_map(&mk, p.k_cache, p, kb)) return rc;
     if (int rc = prefix_cache_map(&mv, p.v_cache, p, kb)) return rc;
     auto run = [&](auto kernel, int nw, int bytes) -> int {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) e = launch_chained(kernel, dim3(p.n_kv_heads * p.own_splits, p.n_seqs), dim3(nw * 32), bytes, stream, mk, mv, p);
+        if (e == cudaSuccess) e = launch_chained(kernel, dim3((unsigned)(p.n_kv_heads * splits), (unsigned)items), dim3(nw * 32), bytes, stream, mk, mv, p);
         if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
         return 0;
     };
-    // the most warps a block with which every block is resident at once; rounds of four-warp blocks where there are too many
-    const int nw = blocks <= sms ? 12 : blocks <= 3l * sms ? 4 : blocks <= 5l * sms ? 2 : blocks <= 10l * sms ? 1 : 4;
-#define MDMA_OWN(DM, KB) (nw == 12 ? run(prefix_own_kernel<DM, KB, 12>, 12, PoSmem<DM, KB, 12>::kBytes) \
-                        : nw == 4 ? run(prefix_own_kernel<DM, KB, 4>, 4, PoSmem<DM, KB, 4>::kBytes) \
-                        : nw == 2 ? run(prefix_own_kernel<DM, KB, 2>, 2, PoSmem<DM, KB, 2>::kBytes) \
-                                  : run(prefix_own_kernel<DM, KB, 1>, 1, PoSmem<DM, KB, 1>::kBytes))
-    return kb == 64 ? MDMA_OWN(64, 64) : p.head_dim <= 64 ? MDMA_OWN(64, 32) : MDMA_OWN(128, 32);
-#undef MDMA_OWN
+    // as many warps a block as leave every block resident at once, two at least (51 sequences x 32 kv heads, own keys and prefixes:
+    // 53 us in rounds of two-warp blocks, 56 with one warp, 67 with four)
+    const int nw = blocks <= sms ? 12 : blocks <= 3l * sms ? 4 : 2;
+#define MDMA_STREAM(DM, KB) (nw == 12 ? run(prefix_stream_kernel<DM, KB, 12, SHARED>, 12, PoSmem<DM, KB, 12>::kBytes) \
+                           : nw == 4 ? run(prefix_stream_kernel<DM, KB, 4, SHARED>, 4, PoSmem<DM, KB, 4>::kBytes) \
+                                     : run(prefix_stream_kernel<DM, KB, 2, SHARED>, 2, PoSmem<DM, KB, 2>::kBytes))
+    return kb == 64 ? MDMA_STREAM(64, 64) : p.head_dim <= 64 ? MDMA_STREAM(64, 32) : MDMA_STREAM(128, 32);
+#undef MDMA_STREAM
 }
 
 static int launch_prefix_tc(const PrefixParams& p, cudaStream_t stream) {
@@ -255,7 +258,9 @@ static int launch_prefix_tc(const PrefixParams& p, cudaStream_t stream) {
 
 using namespace mdma;
 
-extern "C" int mdma_prefix_attention(const long long* words, int n_words, float scale, cudaStream_t stream) {
+// `kind`: who does the prefixes: 0 the tcgen05 kernel (which also takes whole lists of keys), 1 the streaming one, 2 the one for
+// any page size; the own keys of single tokens are streamed where the geometry allows.
+extern "C" int mdma_prefix_attention(const long long* words, int n_words, float scale, int kind, cudaStream_t stream) {
     PrefixParams p;
     if (int rc = prefix_params(words, n_words, scale, &p)) return rc;
     MDMA_REQUIRE(p.head_dim % 16 == 0 && p.head_dim <= 128 && p.group <= kPrRows,
@@ -263,23 +268,23 @@ extern "C" int mdma_prefix_attention(const long long* words, int n_words, float 
                  p.n_heads, p.n_kv_heads, p.head_dim);
     MDMA_REQUIRE(p.q_stride % 8 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache) & 15) == 0, "prefix_attention: rows must be 16-byte aligned");
     MDMA_REQUIRE(((uintptr_t)p.out & 15) == 0, "prefix_attention: the results must be 16-byte aligned");
-    const bool tiled = p.page_size % 64 == 0;
-    MDMA_REQUIRE(!p.whole || tiled, "prefix_attention: whole lists of keys want pages of a multiple of 64 tokens");
+    MDMA_REQUIRE(kind >= 0 && kind <= 2 && (kind == 0 || !p.whole), "prefix_attention: no kernel %d for this step", kind);
+    MDMA_REQUIRE(kind != 0 || p.page_size % 64 == 0, "prefix_attention: the tcgen05 kernel wants pages of a multiple of 64 tokens");
+    MDMA_REQUIRE(kind != 1 || prefix_stream_fits(p), "prefix_attention: the streaming kernel wants single tokens, pages of a multiple of 32 tokens and groups of up to 16 heads");
+    MDMA_REQUIRE(p.pieces > 0 || prefix_stream_fits(p), "prefix_attention: prefixes in no pieces");
     if (p.n_tokens == 0 || p.n_seqs == 0) return 0;
-    if (tiled) {
-        if (int rc = launch_prefix_tc(p, stream)) return rc;
+    p.unit = kind == 0 ? kPtKeys : 64;
+    int sms = 0, dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return fail("prefix_attention: no CUDA device");
+    if (p.pieces > 0) {
+        if (int rc = kind == 0 ? launch_prefix_tc(p, stream) : kind == 1 ? launch_prefix_stream<true>(p, sms, stream) : launch_prefix_rows(p, true, false, stream)) return rc;
         if (p.whole && p.pieces == 1) return 0;
     }
-    if (!p.whole && prefix_own_fits(p)) {
-        if (!tiled)
-            if (int rc = launch_prefix_rows(p, true, false, stream)) return rc;
-        int sms = 0, dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-            return fail("prefix_attention: no CUDA device");
-        if (int rc = launch_prefix_own(p, sms, stream)) return rc;
-        if (p.own_splits == 1) return 0;
-    } else if (!p.whole) {
-        if (int rc = launch_prefix_rows(p, !tiled, true, stream)) return rc;
+    if (!p.whole) {
+        const bool stream_own = prefix_stream_fits(p);
+        if (int rc = stream_own ? launch_prefix_stream<false>(p, sms, stream) : launch_prefix_rows(p, false, true, stream)) return rc;
+        if (stream_own && p.own_splits == 1) return 0;
     }
     return launch_prefix_merge(p, stream);
 }

@@ -1,12 +1,14 @@
-// Single tokens behind shared prefixes: every sequence's own keys, and the join with the parts of its prefix (bfloat16, pages of
-// a multiple of 32 tokens, up to 16 query heads a kv head).
+// Single tokens behind shared prefixes, as streams of keys (bfloat16, pages of a multiple of 32 tokens, up to 16 query heads a kv
+// head): every sequence's own keys with the join of its prefix's parts, and prefixes that few rows share.
 //
 // A block takes one (sequence, kv head): the query heads of the group are the rows of one 16-row tile on mma.sync, its warps take
 // the key tiles in turn, each with a running maximum, sum and output of its own and with its next key tile on the way (TMA)
 // while it multiplies with the values.  It is bound by memory: every key and value is read once.  The kernel of the prefixes
 // runs beside it; only when the own keys are done does the block wait for that kernel, and joins the warps' sums, the
 // prefix's parts (in their order) and the sink.  With `own_splits` > 1 a block takes a piece of the own keys and leaves its sums for
-// the merge.
+// the merge.  Without pieces (`pieces` 0) nothing is shared: a sequence's own keys are all it sees.
+//
+// SHARED: the same over a piece of a prefix, the 16 rows those of several members; every block leaves its sums.
 #pragma once
 #include "mma_tiles.cuh"
 #include "prefix.cuh"
@@ -24,9 +26,9 @@ struct PoSmem {
     static constexpr int kBytes = kTop + (3 * NW * 16 + kPoMaxPieces * 16) * 4;
 };
 
-template <int DMAX, int KB, int NW>
-__global__ void __launch_bounds__(NW * 32, NW >= 8 ? 1 : NW == 4 ? 3 : NW == 2 ? 5 : 10)
-prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams p) {
+template <int DMAX, int KB, int NW, bool SHARED>
+__global__ void __launch_bounds__(NW * 32, NW >= 8 ? 1 : NW == 4 ? 3 : 5)
+prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams p) {
     using L = PoSmem<DMAX, KB, NW>;
     constexpr int kChunks = DMAX / 8, kHalf = KB * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -38,6 +40,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     auto kv_offset = [](int row, int chunk) -> uint32_t {        // 16-byte chunk of a key row inside a tile
         return (uint32_t)((chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
     };
+    // (the kernel of the prefixes lets the next one start only when it has waited itself: that one counts on it)
+    if (SHARED || p.pieces == 0) chain_wait();
     chain_release();
     if (threadIdx.x == 0) {
         for (int w = 0; w < NW; ++w) { ptx::mbar_init(s0 + L::kBars + w * 16, 1); ptx::mbar_init(s0 + L::kBars + w * 16 + 8, 1); }
@@ -45,12 +49,26 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         ptx::fence_mbar_init();
     }
     __syncthreads();
-    const int kvh = blockIdx.x % p.n_kv_heads, split = blockIdx.x / p.n_kv_heads, seq = blockIdx.y;
-    const int token = p.seq_start[seq], pos = p.seq_pos0[seq], skip = p.seq_skip[seq];
-    const int* pages = p.page_table + (size_t)p.seq_slot[seq] * p.max_pages;
+    const int kvh = blockIdx.x % p.n_kv_heads, split = blockIdx.x / p.n_kv_heads;
     const int D = p.head_dim, G = p.group, d_chunks = D / 8, halves = (D + 63) / 64;
-    const int per = ((pos + 1 - skip + p.own_splits - 1) / p.own_splits + KB - 1) / KB * KB;
-    const int lo = skip + split * per, hi = min(pos + 1, lo + per);                   // this block's keys
+    int seq, token = 0, skip = 0, lo, hi, rows = G;                                   // keys [lo, hi) for so many rows
+    PrefixTile tile = {};
+    if (SHARED) {
+        if (!prefix_tile(p, blockIdx.y, 16 / G, tile)) return;
+        const int keys = prefix_piece(tile.len, p.pieces, p.unit);
+        seq = p.group_seq[tile.g]; lo = split * keys; hi = min(tile.len, lo + keys); rows = tile.count * G;
+        if (lo >= hi) return;
+    } else {
+        seq = blockIdx.y;
+        const int end = p.seq_pos0[seq] + 1;
+        token = p.seq_start[seq];
+        skip = p.pieces > 0 ? p.seq_skip[seq] : 0;
+        const int per = ((end - skip + p.own_splits - 1) / p.own_splits + KB - 1) / KB * KB;
+        lo = skip + split * per; hi = min(end, lo + per);
+    }
+    const int* pages = p.page_table + (size_t)p.seq_slot[seq] * p.max_pages;
+    // the token of a row of the tile
+    auto token_of = [&](int r) { return SHARED ? p.toks[tile.first + r / G] : token; };
     const int b1 = hi > lo ? (hi - 1) / KB + 1 : 0;
     int blk = lo / KB + warp;
     auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int at) {      // one lane
@@ -61,11 +79,11 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     };
     if (*abort_flag != 0) blk = b1;
     if (blk < b1 && lane == 0) { load_tile(&map_k, sK, kbar, blk); load_tile(&map_v, sV, vbar, blk); }
-    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (size_t)token * p.q_stride + (size_t)kvh * G * D;
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q);
     for (int i = threadIdx.x; i < 16 * kChunks; i += NW * 32) {  // query rows: zeros beyond the group and the head size
         const int r = i / kChunks, c = i % kChunks;
-        const bool valid = r < G && c < d_chunks;
-        cp_async_16(sQ + tile_offset<DMAX>(r, c), valid ? q + (size_t)r * D + c * 8 : q, valid);
+        const bool valid = r < rows && c < d_chunks;
+        cp_async_16(sQ + tile_offset<DMAX>(r, c), valid ? q + (size_t)token_of(r) * p.q_stride + (size_t)(kvh * G + r % G) * D + c * 8 : q, valid);
     }
     cp_async_commit();
     cp_async_wait<0>();
@@ -172,22 +190,22 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
         for (int n = 0; n < DMAX / 8; ++n) {
             const int d = n * 8 + (lane & 3) * 2;
-            if (r_lo < G) *reinterpret_cast<float2*>(mine + r_lo * L::kRow + d) = make_float2(o[n][0], o[n][1]);
-            if (r_hi < G) *reinterpret_cast<float2*>(mine + r_hi * L::kRow + d) = make_float2(o[n][2], o[n][3]);
+            if (r_lo < rows) *reinterpret_cast<float2*>(mine + r_lo * L::kRow + d) = make_float2(o[n][0], o[n][1]);
+            if (r_hi < rows) *reinterpret_cast<float2*>(mine + r_hi * L::kRow + d) = make_float2(o[n][2], o[n][3]);
         }
         if ((lane & 3) == 0) {
             top[warp * 16 + r_lo] = m_lo; top[(NW + warp) * 16 + r_lo] = l_lo;
             top[warp * 16 + r_hi] = m_hi; top[(NW + warp) * 16 + r_hi] = l_hi;
         }
     }
-    const bool joins = p.own_splits == 1;
-    const int used = joins ? prefix_pieces_used(skip, p.pieces, p.unit) : 0, slots = p.pieces + p.own_splits;
-    const size_t row0 = (size_t)token * p.n_heads + kvh * G;
-    chain_wait();                                                // the prefixes' parts are there, and all that was waited for before them
+    const bool joins = !SHARED && p.own_splits == 1;
+    const int used = joins && p.pieces > 0 ? prefix_pieces_used(skip, p.pieces, p.unit) : 0, slots = p.pieces + p.own_splits;
+    auto row_of = [&](int r) { return (size_t)token_of(r) * p.n_heads + kvh * G + r % G; };
+    if (!SHARED) chain_wait();                                   // the prefixes' parts are there, and all that was waited for before them
     __syncthreads();
-    if ((int)threadIdx.x < G) {                                  // a row a thread: its maximum, its sum, the shares
+    if ((int)threadIdx.x < rows) {                               // a row a thread: its maximum, its sum, the shares
         const int r = threadIdx.x;
-        const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (row0 + r) * slots;
+        const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row_of(r) * slots;
         float m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) m = fmaxf(m, top[w * 16 + r]);
@@ -209,31 +227,30 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         top[r] = m; top[NW * 16 + r] = l;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < G * (D / 2); i += NW * 32) {
-        const int r = i / (D / 2), d = 2 * (i - r * (D / 2));
+    for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 32) {
+        const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
         const float l = top[NW * 16 + r];
-        float2 acc = make_float2(0.f, 0.f);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto join = [&](float f, const float4& x) {
+            if (f != -1.f) { acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w); }
+        };
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = top[(2 * NW + w) * 16 + r];
-            if (f != -1.f) {
-                const float2 x = *reinterpret_cast<const float2*>(comb + ((size_t)w * 16 + r) * L::kRow + d);
-                acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y);
-            }
-        }
-        const float* part = p.part_o + (row0 + r) * slots * D + d;
-#pragma unroll 4
-        for (int s = 0; s < used; ++s) {
-            const float f = share[s * 16 + r];
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(part + (size_t)s * D));
-            if (f != -1.f) { acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); }
+        for (int w = 0; w < NW; ++w) join(top[(2 * NW + w) * 16 + r], *reinterpret_cast<const float4*>(comb + ((size_t)w * 16 + r) * L::kRow + d));
+        const size_t row = row_of(r);
+        const float* part = p.part_o + row * slots * D + d;
+        for (int s0 = 0; s0 < used; s0 += 8) {                   // eight parts in flight
+            float4 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = __ldcg(reinterpret_cast<const float4*>(part + (size_t)min(s0 + u, used - 1) * D));
+#pragma unroll
+            for (int u = 0; u < 8; ++u) if (s0 + u < used) join(share[(s0 + u) * 16 + r], x[u]);
         }
         if (joins) {
-            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + (row0 + r) * D + d;
-            *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(acc.x / l, acc.y / l);
+            __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x / l, acc.y / l), __floats2bfloat162_rn(acc.z / l, acc.w / l)};
+            *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * D + d) = *reinterpret_cast<const uint2*>(y);
         } else {
-            const size_t slot = (row0 + r) * slots + p.pieces + split;
-            *reinterpret_cast<float2*>(p.part_o + slot * D + d) = acc;
+            const size_t slot = row * slots + (SHARED ? 0 : p.pieces) + split;
+            *reinterpret_cast<float4*>(p.part_o + slot * D + d) = acc;
             if (d == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(top[r], l);
         }
     }

@@ -264,7 +264,7 @@ extern "C" int mdma_prefix_attention_simple(const long long* words, int n_words,
     PrefixParams p;
     if (int rc = prefix_params(words, n_words, scale, &p)) return rc;
     p.unit = kPsKeys;
-    MDMA_REQUIRE(!p.whole, "prefix_attention: whole lists of keys are the tensor-core kernel's");
+    MDMA_REQUIRE(!p.whole && p.pieces > 0, "prefix_attention: %d and %d pieces are none of this kernel's", p.pieces, p.own_splits);
     if (p.n_tokens == 0 || p.n_seqs == 0) return 0;
     MDMA_DISPATCH_DTYPE(dtype, T, return launch_prefix_simple<T>(p, prefix_rows, own_rows, stream));
     return 0;

@@ -90,7 +90,7 @@ prefix_merge_kernel(const PrefixParams p) {
     const int lane = threadIdx.x & 31;
     if (row >= (long)p.n_tokens * p.n_heads) return;
     const int slots = p.pieces + p.own_splits, D = p.head_dim;
-    const int used = p.whole ? p.pieces : prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces, p.unit), parts = used + p.own_splits;
+    const int used = p.whole || p.pieces == 0 ? p.pieces : prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces, p.unit), parts = used + p.own_splits;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * slots;
     auto slot_of = [&](int s) { return s < used ? s : p.pieces + s - used; };
     float2 mine[2];
@@ -157,12 +157,12 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     MDMA_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0, "prefix_attention: %d heads over %d kv heads", p.n_heads, p.n_kv_heads);
     MDMA_REQUIRE(p.head_dim > 0 && p.head_dim <= 256, "prefix_attention: head_dim %d is beyond the limit of 256", p.head_dim);
     MDMA_REQUIRE(p.page_table && p.page_size > 0 && p.max_pages > 0, "prefix_attention: bad cache geometry");
-    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 1 && p.own_splits >= 0, "prefix_attention: bad sizes");
+    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 0 && p.own_splits >= 0 && p.pieces + p.own_splits > 0, "prefix_attention: bad sizes");
     MDMA_REQUIRE(p.pieces <= 32 && p.own_splits <= 32, "prefix_attention: %d and %d pieces are beyond the limit of 32", p.pieces, p.own_splits);
     MDMA_REQUIRE(scale > 0.f, "prefix_attention: the score scale must be positive");
     p.group = p.n_heads / p.n_kv_heads;
     p.whole = p.own_splits == 0; p.unit = 128;
-    const long long slots = p.whole && p.pieces == 1 ? 0 : (long long)p.n_tokens * p.n_heads * (p.pieces + p.own_splits), need = slots ? slots * (p.head_dim + 2) + 4 : 0;
+    const long long slots = p.pieces + p.own_splits == 1 ? 0 : (long long)p.n_tokens * p.n_heads * (p.pieces + p.own_splits), need = slots ? slots * (p.head_dim + 2) + 4 : 0;
     MDMA_REQUIRE(need == 0 || (scratch && floats >= need), "prefix_attention: %lld floats of scratch are needed, %lld given", need, floats);
     MDMA_REQUIRE(((uintptr_t)scratch & 15) == 0, "prefix_attention: the scratch must be 16-byte aligned");
     // pairs first, so that they lie at multiples of 8 bytes and the sums behind them of 16, whatever the head size

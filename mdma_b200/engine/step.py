@@ -142,13 +142,13 @@ def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_cont
 
     from .. import ops, ops_tensor
     ctx = SimpleNamespace(max_new=1, n_seqs=max_slots, n_tokens=max_slots, most_seqs=max_slots)
-    most = SimpleNamespace(most_len=max_context, most_own=max_context)
+    most = SimpleNamespace(most_len=max_context, most_own=max_context, most_tokens=max_slots, n_groups=1)
     need = 0
     for part in model.all_parts():
         for heads, kv_heads, head_dim in getattr(part, "prefix_shapes", list)():
             parts = sum(ops.prefix_plan(ctx, most, heads, kv_heads))
             if dtype == torch.bfloat16 and ops_tensor.attention_supported(heads, kv_heads, head_dim):
-                parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, sms, page_size)))
+                parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, head_dim, sms, page_size)[:2]))
             need = max(need, ops.prefix_scratch_floats(max_slots, heads, parts, head_dim))
     return need
 

@@ -638,6 +638,10 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
 
 
 # ---- attention of sequences that share their beginning (csrc/attention_prefix.cu) ------------------------------------------
+PREFIX_LEAST_BYTES = 100 << 20
+PREFIX_STREAM_ROWS = 16
+
+
 def prefix_own_splits(seqs: int, n_heads: int, n_kv_heads: int, most_own: int, sms: int) -> int:
     """Into how many pieces a single token's own keys are cut: one block a (sequence, kv head) joins everything itself unless
     the blocks leave most of the device idle and have more than a thousand keys each."""
@@ -648,22 +652,33 @@ def prefix_own_splits(seqs: int, n_heads: int, n_kv_heads: int, most_own: int, s
     return max(1, min(sms // (seqs * n_kv_heads), most_own // 512, 16))
 
 
-def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int, page_size: int) -> tuple[int, int]:
-    """(pieces of a prefix, pieces of a sequence's own keys); of single tokens from the most sequences the engine can hold (see
-    `ops.prefix_plan`).  (n, 0): prefix and own keys are one list in n pieces."""
-    one = ctx.max_new == 1
+# who does the prefixes (csrc/attention_prefix.cu)
+PREFIX_TC, PREFIX_STREAM, PREFIX_ROWS = 0, 1, 2
+
+
+def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, page_size: int) -> tuple[int, int, int]:
+    """(pieces of a prefix, pieces of a sequence's own keys, kernel of the prefixes); of single tokens from the most sequences the
+    engine can hold (see `ops.prefix_plan`).  (n, 0, ..): prefix and own keys are one list in n pieces; (0, n, ..): every
+    sequence reads its prefix by itself."""
+    one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
-    if page_size % 64 == 0:                       # the tcgen05 kernel: 256 query rows a block, one block an SM
-        tile_tokens = 2 * (128 // (n_heads // n_kv_heads))
+    streams = one and page_size % 32 == 0 and group <= 16
+    if streams and seqs * g.most_len * n_kv_heads * head_dim * 4 <= PREFIX_LEAST_BYTES:
+        return 0, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_len + g.most_own, sms), PREFIX_STREAM
+    rows = group * (getattr(ctx, "most_seqs", None) or g.most_tokens)
+    if streams and (rows <= PREFIX_STREAM_ROWS or page_size % 64):
+        tiles = -(-seqs // (16 // group)) * n_kv_heads
+        pieces = max(1, min(2 * sms // tiles, 32, -(-g.most_len // 256)))
+        return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_STREAM
+    if page_size % 64 == 0:                       # 256 query rows a block, one block an SM
+        tile_tokens = 2 * (128 // group)
         tiles = -(-seqs // tile_tokens) if one else ctx.n_tokens // tile_tokens + g.n_groups
         most = sms // (tiles * n_kv_heads)
         if not one:
-            return max(1, min(most, 32, (g.most_len + g.most_own) // 256)), 0
-        return max(1, min(most, 32, -(-g.most_len // 128))), prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms)
-    if one and page_size % 32 == 0 and n_heads // n_kv_heads <= 16:
-        return (ops.prefix_split(64, 2 * sms, seqs, seqs, 1, g.most_len, 0, n_heads, n_kv_heads)[0],
-                prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms))
-    return ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
+            return max(1, min(most, 32, (g.most_len + g.most_own) // 256)), 0, PREFIX_TC
+        return max(1, min(most, 32, -(-g.most_len // 128))), prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_TC
+    pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
+    return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms) if streams else own, PREFIX_ROWS
 
 
 def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
@@ -681,7 +696,7 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     st = st or _device_state(q.device)
     flush_pending(q.device, st)
     g = ctx.prefix
-    pieces, own = prefix_plan(ctx, g, n_heads, n_kv_heads, st.sms, view.page_size)
+    pieces, own, kind = prefix_plan(ctx, g, n_heads, n_kv_heads, head_dim, st.sms, view.page_size)
     need = ops.prefix_scratch_floats(ctx.n_tokens, n_heads, pieces + own, head_dim) if pieces + own > 1 else 0
     if own_st is not None:
         st.need(need, "attention over shared prefixes")
@@ -689,4 +704,5 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     else:
         scratch = torch.empty(need, dtype=torch.float32, device=q.device)
     words = ops.prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sink_log2, st.status, True)
-    _call("tensor", "mdma_prefix_attention", words, _i(32), _f(scale), _stream(), launches=2)
+    _call("tensor", "mdma_prefix_attention", words, _i(32), _f(scale), _i(kind), _stream(),
+          launches=(pieces > 0) + (own > 0) + (pieces > 1 if own == 0 else own > 1 or ctx.max_new > 1 or n_heads // n_kv_heads > 16 or view.page_size % 32 != 0))

@@ -276,8 +276,11 @@ class Attention(Part):
             return False
         if self._fast_ok:
             from .. import ops_tensor
-            parts = sum(ops_tensor.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads, self.rt.tc.sms if self.rt.tc is not None else 148,
-                                               view.page_size))
+            pieces, own, _ = ops_tensor.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads, self.head_dim,
+                                                    self.rt.tc.sms if self.rt.tc is not None else 148, view.page_size)
+            if pieces == 0:              # every sequence by itself: so do the kernels of steps that share nothing
+                return False
+            parts = pieces + own
             if parts == 1:
                 return True
             scratch = self.rt.tc.scratch if self.rt.tc is not None and not self.rt.tc.growable else None
