@@ -214,7 +214,7 @@ static int prefix_cache_map(CUtensorMap* out, const void* cache, const PrefixPar
 }
 
 static bool prefix_stream_fits(const PrefixParams& p) {
-    return p.max_new == 1 && p.group <= 16 && p.page_size % 32 == 0 && p.pieces <= kPoMaxPieces && p.own_splits >= 1;
+    return p.max_new == 1 && p.n_tokens == p.n_seqs && p.group <= 16 && p.page_size % 32 == 0 && p.pieces <= kPoMaxPieces && p.own_splits >= 1;
 }
 // The sequences' own keys, or the prefixes.
 template <bool SHARED>

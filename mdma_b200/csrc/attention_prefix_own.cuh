@@ -23,7 +23,7 @@ struct PoSmem {
     static constexpr int kTile = KB * DMAX * 2, kRow = DMAX + 8;                      // bytes of a tile; floats of a warp's row of sums
     static constexpr int kTiles = NW * 2 * kTile, kComb = NW * 16 * kRow * 4;
     static constexpr int kQ = kTiles > kComb ? kTiles : kComb, kBars = kQ + 16 * DMAX * 2, kTop = kBars + NW * 16 + 16;
-    static constexpr int kBytes = kTop + (3 * NW * 16 + kPoMaxPieces * 16) * 4;
+    static constexpr int kBytes = kTop + (3 * NW * 16 + kPoMaxPieces * 16 * 3) * 4;
 };
 
 template <int DMAX, int KB, int NW, bool SHARED>
@@ -61,7 +61,7 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     } else {
         seq = blockIdx.y;
         const int end = p.seq_pos0[seq] + 1;
-        token = p.seq_start[seq];
+        token = seq;                                             // (every sequence brings one)
         skip = p.pieces > 0 ? p.seq_skip[seq] : 0;
         const int per = ((end - skip + p.own_splits - 1) / p.own_splits + KB - 1) / KB * KB;
         lo = skip + split * per; hi = min(end, lo + per);
@@ -203,13 +203,20 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     auto row_of = [&](int r) { return (size_t)token_of(r) * p.n_heads + kvh * G + r % G; };
     if (!SHARED) chain_wait();                                   // the prefixes' parts are there, and all that was waited for before them
     __syncthreads();
+    float2* parts = reinterpret_cast<float2*>(share + kPoMaxPieces * 16);             // [pieces][16] maxima and sums of the prefix's parts
+    if (used > 0) {
+        for (int i = threadIdx.x; i < used * rows; i += NW * 32) {
+            const int s = i % used, r = i / used;
+            parts[s * 16 + r] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + row_of(r) * slots + s);
+        }
+        __syncthreads();
+    }
     if ((int)threadIdx.x < rows) {                               // a row a thread: its maximum, its sum, the shares
         const int r = threadIdx.x;
-        const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row_of(r) * slots;
         float m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) m = fmaxf(m, top[w * 16 + r]);
-        for (int s = 0; s < used; ++s) m = fmaxf(m, __ldcg(&ml[s]).x);
+        for (int s = 0; s < used; ++s) m = fmaxf(m, parts[s * 16 + r].x);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float mw = top[w * 16 + r];
@@ -218,7 +225,7 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             top[(2 * NW + w) * 16 + r] = f;
         }
         for (int s = 0; s < used; ++s) {
-            const float2 x = __ldcg(&ml[s]);
+            const float2 x = parts[s * 16 + r];
             float f = -1.f;
             if (x.x != -INFINITY) { f = exp2f(x.x - m); l += f * x.y; }
             share[s * 16 + r] = f;

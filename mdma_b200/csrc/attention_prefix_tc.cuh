@@ -31,6 +31,7 @@ namespace mdma {
 constexpr int kPtRows = 128, kPtKeys = 128, kPtThreads = 320, kPtMaxTokens = 2 * kPtRows;
 constexpr int kPtHalf = kPtRows * 128;                           // 128 rows (or keys) x 64 numbers
 constexpr int kPtSlot = 2 * kPtHalf;
+constexpr int kPtStage = 132;                                   // floats from row to row of results on their way out
 constexpr int kPtSmemK = 2 * kPtSlot, kPtSmemV = kPtSmemK + 2 * kPtSlot, kPtSmemBars = kPtSmemV + 2 * kPtSlot;
 struct PtSegment { int seq, key0, key1, tok0, toks, block0; };  // keys [key0, key1) for the tile's tokens [tok0, tok0 + toks); its first block
 constexpr int kPtSmemSegs = kPtSmemBars + 256;
@@ -288,26 +289,24 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         // ---- softmax: a row a thread --------------------------------------------------------------------------------
         const int t = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16, tmem_s = tmem + t * 128 + lanes, tmem_o = tmem + 256 + t * 128 + lanes;
-        {
-            // queries into shared memory, 128-byte rows with the 128-byte swizzle, zeros beyond the tile's rows
-            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q);
-            const int chunks = halves * 8, tokens = min(count - t * tt, tt);
-            if (tokens > 0) {
-#pragma unroll 4
-                for (int i = threadIdx.x & 127; i < kPtRows * chunks; i += 128) {
-                    const int qr = i / chunks, c = i % chunks, qt = qr / G;
-                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    if (qt < tokens && c * 8 < D)
-                        x = *reinterpret_cast<const uint4*>(q + (size_t)p.toks[tile.first + t * tt + qt] * p.q_stride + (size_t)(kvh * G + qr % G) * D + c * 8);
-                    *reinterpret_cast<uint4*>(smem + t * kPtSlot + (c >> 3) * kPtHalf + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = x;
-                }
-                ptx::fence_proxy_async_shared();
-            }
-            ptx::mbar_arrive(q_full);
-        }
         const int tok = t * tt + r / G;                          // of the block's tokens
         const bool row_valid = r / G < tt && tok < count;
         const int token = row_valid ? p.toks[tile.first + tok] : -1;
+        if (t == 0 || count > tt) {
+            // the row's query into shared memory, 128-byte rows with the 128-byte swizzle, zeros beyond the tile's rows (a row a
+            // thread, all of it in flight: with the rows' chunks dealt out over the threads, each asking for its row's token first, it
+            // took 3 to 9 us)
+            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (size_t)max(token, 0) * p.q_stride + (size_t)(kvh * G + r % G) * D;
+            uint4 x[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+                x[c] = row_valid && c * 8 < D ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+                if (c < halves * 8) *reinterpret_cast<uint4*>(smem + t * kPtSlot + (c >> 3) * kPtHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[c];
+            ptx::fence_proxy_async_shared();
+        }
+        ptx::mbar_arrive(q_full);
         const int pos = p.whole && row_valid ? p.seq_pos0[p.tok_seq[token]] + token - p.seq_start[p.tok_seq[token]] : 0;
         float m_ref = -INFINITY, l = 0.f;
         {
@@ -432,50 +431,42 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(s_full(t), seen & 1, abort_flag));
         if (ok) {
             ptx::tc_fence_after_sync();
-            const size_t row = (size_t)(row_valid ? token : 0) * p.n_heads + kvh * G + r % G;
-            if (p.whole && p.pieces == 1) {
+            // Rows go out through shared memory (every product has read its operands): written by the thread that holds it, a
+            // row's pieces of 16 bytes would lie 512 bytes and more apart from the next thread's.
+            const bool final = p.whole && p.pieces == 1;
+            const size_t row = (size_t)max(token, 0) * p.n_heads + kvh * G + r % G, at = row * (p.pieces + p.own_splits) + split;
+            float inv = 1.0f;
+            if (final) {
                 if (p.sinks) l += exp2f(p.sinks[kvh * G + r % G] * p.sink_rate - m_ref);
-                const float inv = 1.0f / l;
-                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + row * D;
+                inv = 1.0f / l;
+            } else if (row_valid) {
+                *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
+            }
+            float* stage = reinterpret_cast<float*>(smem) + warp * 32 * kPtStage;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c * 32 < D) {
-                        float v[32];
-                        ptx::tmem_load_32_nowait(tmem_o + c * 32, v);
-                        ptx::tmem_load_wait();
-                        if (row_valid) {
+            for (int c = 0; c < 4; ++c) {
+                if (c * 32 < D) {
+                    float v[32];
+                    ptx::tmem_load_32_nowait(tmem_o + c * 32, v);
+                    ptx::tmem_load_wait();
 #pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                if (c * 32 + q * 8 < D) {
-                                    uint32_t x[4];
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[q * 8 + 2 * i] * inv, v[q * 8 + 2 * i + 1] * inv);
-                                        x[i] = *reinterpret_cast<const uint32_t*>(&b2);
-                                    }
-                                    *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = make_uint4(x[0], x[1], x[2], x[3]);
-                                }
-                        }
-                    }
+                    for (int q = 0; q < 8; ++q)
+                        *reinterpret_cast<float4*>(stage + lane * kPtStage + c * 32 + q * 4) = make_float4(v[4 * q] * inv, v[4 * q + 1] * inv, v[4 * q + 2] * inv, v[4 * q + 3] * inv);
                 }
-            } else {
-                const size_t at = row * (p.pieces + p.own_splits) + split;
-                float* dst = p.part_o + at * D;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c * 32 < D) {
-                        float v[32];
-                        ptx::tmem_load_32_nowait(tmem_o + c * 32, v);
-                        ptx::tmem_load_wait();
-                        if (row_valid) {
-#pragma unroll
-                            for (int q = 0; q < 8; ++q)
-                                if (c * 32 + q * 4 < D)
-                                    *reinterpret_cast<float4*>(dst + c * 32 + q * 4) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                        }
-                    }
+            }
+            __syncwarp();
+            const uint64_t mine = row_valid ? (final ? row : at) : ~0ull;
+#pragma unroll 4
+            for (int i = 0; i < 32; ++i) {
+                const uint64_t to = __shfl_sync(0xffffffffu, mine, i);
+                if (to == ~0ull || lane * 4 >= D) continue;
+                const float4 x = *reinterpret_cast<const float4*>(stage + i * kPtStage + lane * 4);
+                if (final) {
+                    const __nv_bfloat162 y[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + to * D + lane * 4) = *reinterpret_cast<const uint2*>(y);
+                } else {
+                    *reinterpret_cast<float4*>(p.part_o + to * D + lane * 4) = x;
                 }
-                if (row_valid) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
             }
             ptx::tc_fence_before_sync();
         }

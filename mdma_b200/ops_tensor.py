@@ -662,7 +662,7 @@ def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, 
     sequence reads its prefix by itself."""
     one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
-    streams = one and page_size % 32 == 0 and group <= 16
+    streams = one and page_size % 32 == 0 and group <= 16 and ctx.n_tokens == ctx.n_seqs
     if streams and seqs * g.most_len * n_kv_heads * head_dim * 4 <= PREFIX_LEAST_BYTES:
         return 0, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_len + g.most_own, sms), PREFIX_STREAM
     rows = group * (getattr(ctx, "most_seqs", None) or g.most_tokens)
