@@ -164,8 +164,7 @@ prefix_rows_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
 }
 
 static int launch_prefix_merge(const PrefixParams& p, cudaStream_t stream) {
-    const long rows = (long)p.n_tokens * p.n_heads;
-    const cudaError_t e = launch_chained(prefix_merge_kernel<__nv_bfloat16>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, p);
+    const cudaError_t e = launch_chained(prefix_merge_kernel<__nv_bfloat16>, dim3(prefix_merge_blocks(p)), dim3(128), 0, stream, p);
     if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }

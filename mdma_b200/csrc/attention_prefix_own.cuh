@@ -23,7 +23,7 @@ struct PoSmem {
     static constexpr int kTile = KB * DMAX * 2, kRow = DMAX + 8;                      // bytes of a tile; floats of a warp's row of sums
     static constexpr int kTiles = NW * 2 * kTile, kComb = NW * 16 * kRow * 4;
     static constexpr int kQ = kTiles > kComb ? kTiles : kComb, kBars = kQ + 16 * DMAX * 2, kTop = kBars + NW * 16 + 16;
-    static constexpr int kBytes = kTop + (3 * NW * 16 + kPoMaxPieces * 16 * 3) * 4;
+    static constexpr int kBytes = kTop + (3 * NW + kPoMaxPieces + 2) * 16 * 4;
 };
 
 template <int DMAX, int KB, int NW, bool SHARED>
@@ -182,8 +182,9 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     // ---- join: warps in their order, then the prefix's parts in theirs -----------------------------------------------
     __syncthreads();                                             // the tiles are read: their place takes the warps' sums
     float* comb = reinterpret_cast<float*>(smem);
-    float* top = reinterpret_cast<float*>(smem + L::kTop);       // [NW][16] maxima, [NW][16] sums, [NW][16] shares
-    float* share = top + 3 * NW * 16;                            // [pieces][16] shares of the prefix's parts
+    float* top = reinterpret_cast<float*>(smem + L::kTop);       // [NW][16] maxima, [NW][16] sums of the warps
+    float* share = top + 2 * NW * 16;                            // [NW + pieces][16] shares of the warps and of the prefix's parts
+    float *row_m = share + (NW + kPoMaxPieces) * 16, *row_l = row_m + 16;
     {
         float* mine = comb + (size_t)warp * 16 * L::kRow;
         const int r_lo = lane >> 2, r_hi = r_lo + 8;
@@ -203,54 +204,51 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     auto row_of = [&](int r) { return (size_t)token_of(r) * p.n_heads + kvh * G + r % G; };
     if (!SHARED) chain_wait();                                   // the prefixes' parts are there, and all that was waited for before them
     __syncthreads();
-    float2* parts = reinterpret_cast<float2*>(share + kPoMaxPieces * 16);             // [pieces][16] maxima and sums of the prefix's parts
-    if (used > 0) {
-        for (int i = threadIdx.x; i < used * rows; i += NW * 32) {
-            const int s = i % used, r = i / used;
-            parts[s * 16 + r] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + row_of(r) * slots + s);
-        }
-        __syncthreads();
-    }
-    if ((int)threadIdx.x < rows) {                               // a row a thread: its maximum, its sum, the shares
-        const int r = threadIdx.x;
-        float m = -INFINITY, l = 0.f;
+    // a warp a row: the maximum of the warps' and the parts' maxima, everyone's share, the sum (a lane a contribution, up to two)
+    for (int r = warp; r < rows; r += NW) {
+        const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row_of(r) * slots;
+        float2 mine[2];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) m = fmaxf(m, top[w * 16 + r]);
-        for (int s = 0; s < used; ++s) m = fmaxf(m, parts[s * 16 + r].x);
+        for (int u = 0; u < 2; ++u) {
+            const int i = u * 32 + lane;
+            mine[u] = i < NW ? make_float2(top[i * 16 + r], top[(NW + i) * 16 + r]) : i < NW + used ? __ldcg(ml + i - NW) : make_float2(-INFINITY, 0.f);
+        }
+        const float m = warp_max(fmaxf(mine[0].x, mine[1].x));
+        float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float mw = top[w * 16 + r];
-            float f = -1.f;                                      // a warp without keys has no share
-            if (mw != -INFINITY) { f = exp2f(mw - m); l += f * top[(NW + w) * 16 + r]; }
-            top[(2 * NW + w) * 16 + r] = f;
+        for (int u = 0; u < 2; ++u) {
+            const float f = mine[u].x == -INFINITY ? -1.f : exp2f(mine[u].x - m);     // who has no keys has no share
+            if (f >= 0.f) l += f * mine[u].y;
+            if (u * 32 + lane < NW + used) share[(u * 32 + lane) * 16 + r] = f;
         }
-        for (int s = 0; s < used; ++s) {
-            const float2 x = parts[s * 16 + r];
-            float f = -1.f;
-            if (x.x != -INFINITY) { f = exp2f(x.x - m); l += f * x.y; }
-            share[s * 16 + r] = f;
+        l = warp_sum(l);
+        if (lane == 0) {
+            if (joins && p.sinks) l += exp2f(p.sinks[kvh * G + r % G] * p.sink_rate - m);
+            row_m[r] = m; row_l[r] = l;
         }
-        if (joins && p.sinks) l += exp2f(p.sinks[kvh * G + r] * p.sink_rate - m);
-        top[r] = m; top[NW * 16 + r] = l;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 32) {
         const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
-        const float l = top[NW * 16 + r];
+        const float l = row_l[r];
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         auto join = [&](float f, const float4& x) {
-            if (f != -1.f) { acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w); }
+            if (f >= 0.f) { acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w); }
         };
-#pragma unroll
-        for (int w = 0; w < NW; ++w) join(top[(2 * NW + w) * 16 + r], *reinterpret_cast<const float4*>(comb + ((size_t)w * 16 + r) * L::kRow + d));
         const size_t row = row_of(r);
         const float* part = p.part_o + row * slots * D + d;
-        for (int s0 = 0; s0 < used; s0 += 8) {                   // eight parts in flight
-            float4 x[8];
+        float4 x[8];
+        auto fetch = [&](int s0) {                               // eight parts in flight
 #pragma unroll
             for (int u = 0; u < 8; ++u) x[u] = __ldcg(reinterpret_cast<const float4*>(part + (size_t)min(s0 + u, used - 1) * D));
+        };
+        if (used > 0) fetch(0);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) if (s0 + u < used) join(share[(s0 + u) * 16 + r], x[u]);
+        for (int w = 0; w < NW; ++w) join(share[w * 16 + r], *reinterpret_cast<const float4*>(comb + ((size_t)w * 16 + r) * L::kRow + d));
+        for (int s0 = 0; s0 < used; s0 += 8) {
+            if (s0 > 0) fetch(s0);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) if (s0 + u < used) join(share[(NW + s0 + u) * 16 + r], x[u]);
         }
         if (joins) {
             __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x / l, acc.y / l), __floats2bfloat162_rn(acc.z / l, acc.w / l)};
@@ -258,7 +256,7 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         } else {
             const size_t slot = row * slots + (SHARED ? 0 : p.pieces) + split;
             *reinterpret_cast<float4*>(p.part_o + slot * D + d) = acc;
-            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(top[r], l);
+            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(row_m[r], l);
         }
     }
     if (threadIdx.x == 0 && *abort_flag && p.status) atomicExch(p.status, 8);

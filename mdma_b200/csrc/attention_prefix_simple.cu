@@ -31,6 +31,7 @@ prefix_simple_kernel(const PrefixParams p, int own_tiles, int wide) {
     float* skv = sq + kRows * kPitch;                // [stage][keys, values][32][pitch]
     float* sp = skv + 4 * kPsKeys * kPitch;          // [rows][33]
     __shared__ int row_token[kRows], row_last[kRows];
+    __shared__ long place[2][kPsKeys];
 
     const int G = p.group, D = p.head_dim, kvh = blockIdx.y, tt = kRows / G > 0 ? kRows / G : 1;
     const int parts = (G + kRows - 1) / kRows, heads_at = (int)blockIdx.z % parts * kRows;       // first head of the group in this tile
@@ -65,36 +66,40 @@ prefix_simple_kernel(const PrefixParams p, int own_tiles, int wide) {
     const int* pages = p.page_table + (size_t)p.seq_slot[seq] * p.max_pages;
     const T* kc = reinterpret_cast<const T*>(p.k_cache);
     const T* vc = reinterpret_cast<const T*>(p.v_cache);
-    auto load = [&](int key0, int stage) {
+    // where the rows of a tile lie: looked up by a thread a row, one tile before the tile is fetched
+    auto find = [&](int key0, int which) {
+        const int key = key0 + (int)threadIdx.x;
+        if ((int)threadIdx.x < kPsKeys)
+            place[which][threadIdx.x] = key < hi ? (((long)pages[key / p.page_size] * p.page_size + key % p.page_size) * p.n_kv_heads + kvh) * D : -1;
+    };
+    auto load = [&](int stage) {
         float* dk = skv + stage * 2 * kPsKeys * kPitch;
         float* dv = dk + kPsKeys * kPitch;
         if (wide) {                                  // floats, 16 bytes at a time, asynchronously
             const int chunks = kWidth / 4;
 #pragma unroll 4
             for (int i = threadIdx.x; i < kPsKeys * chunks; i += kPsThreads) {
-                const int r = i / chunks, c = i % chunks, key = key0 + r;
-                const bool valid = key < hi && c * 4 < D;          // rows beyond belong to nobody: zeros instead
-                size_t at = 0;
-                if (valid) at = (((size_t)pages[key / p.page_size] * p.page_size + key % p.page_size) * p.n_kv_heads + kvh) * D + c * 4;
+                const int r = i / chunks, c = i % chunks;
+                const bool valid = place[stage][r] >= 0 && c * 4 < D;      // rows beyond belong to nobody: zeros instead
+                const long at = valid ? place[stage][r] + c * 4 : 0;
                 cp_async_16((uint32_t)__cvta_generic_to_shared(dk + r * kPitch + c * 4), kc + at, valid);
                 cp_async_16((uint32_t)__cvta_generic_to_shared(dv + r * kPitch + c * 4), vc + at, valid);
             }
         } else {
 #pragma unroll 4
             for (int i = threadIdx.x; i < kPsKeys * kWidth; i += kPsThreads) {
-                const int r = i / kWidth, d = i % kWidth, key = key0 + r;
+                const int r = i / kWidth, d = i % kWidth;
                 float k = 0.f, v = 0.f;
-                if (key < hi && d < D) {
-                    const size_t at = (((size_t)pages[key / p.page_size] * p.page_size + key % p.page_size) * p.n_kv_heads + kvh) * D + d;
-                    k = to_float(kc[at]); v = to_float(vc[at]);
-                }
+                if (place[stage][r] >= 0 && d < D) { k = to_float(kc[place[stage][r] + d]); v = to_float(vc[place[stage][r] + d]); }
                 dk[r * kPitch + d] = k; dv[r * kPitch + d] = v;
             }
         }
         cp_async_commit();
     };
-    if (lo < hi) load(lo, 0);
-    __syncthreads();                                 // the rows' tokens are known
+    find(lo, 0);
+    find(lo + kPsKeys, 1);
+    __syncthreads();                                 // the rows' tokens and the first keys' places are known
+    if (lo < hi) load(0);
     const T* q = reinterpret_cast<const T*>(p.q);
     if (wide) {
         constexpr int chunks = kWidth / 4;
@@ -123,9 +128,10 @@ prefix_simple_kernel(const PrefixParams p, int own_tiles, int wide) {
     const uint32_t group = ((1u << KG) - 1u) << ((threadIdx.x & 31) / KG * KG);      // this group's lanes
     int stage = 0;
     for (int key0 = lo; key0 < hi; key0 += kPsKeys, stage ^= 1) {
-        if (key0 + kPsKeys < hi) load(key0 + kPsKeys, stage ^ 1); else cp_async_commit();
+        if (key0 + kPsKeys < hi) load(stage ^ 1); else cp_async_commit();
         cp_async_wait<1>();
         __syncthreads();
+        find(key0 + 2 * kPsKeys, stage);             // (the places of the keys that are here have been used)
         const float* sk = skv + stage * 2 * kPsKeys * kPitch;
         const float* sv = sk + kPsKeys * kPitch;
         if (working) {
@@ -238,9 +244,9 @@ static int launch_prefix_simple_rows(const PrefixParams& p, bool own, int rows, 
         return D <= 64 ? launch_prefix_simple_as<T, 8, 1, 1>(p, own, wide, stream) : D <= 128 ? launch_prefix_simple_as<T, 8, 1, 2>(p, own, wide, stream)
                                                                                            : launch_prefix_simple_as<T, 8, 1, 4>(p, own, wide, stream);
     if (rows <= 32 || D > 128)
-        return D <= 64 ? launch_prefix_simple_as<T, 16, 2, 2>(p, own, wide, stream) : D <= 128 ? launch_prefix_simple_as<T, 16, 2, 4>(p, own, wide, stream)
+        return D <= 64 ? launch_prefix_simple_as<T, 16, 2, 2>(p, own, wide, stream) : D <= 96 ? launch_prefix_simple_as<T, 16, 2, 3>(p, own, wide, stream) : D <= 128 ? launch_prefix_simple_as<T, 16, 2, 4>(p, own, wide, stream)
                                                                                            : launch_prefix_simple_as<T, 16, 2, 8>(p, own, wide, stream);
-    return D <= 64 ? launch_prefix_simple_as<T, 16, 4, 2>(p, own, wide, stream) : launch_prefix_simple_as<T, 16, 4, 4>(p, own, wide, stream);
+    return D <= 64 ? launch_prefix_simple_as<T, 16, 4, 2>(p, own, wide, stream) : D <= 96 ? launch_prefix_simple_as<T, 16, 4, 3>(p, own, wide, stream) : launch_prefix_simple_as<T, 16, 4, 4>(p, own, wide, stream);
 }
 
 template <typename T>
@@ -249,8 +255,7 @@ static int launch_prefix_simple(const PrefixParams& p, int prefix_rows, int own_
                      (((uintptr_t)p.k_cache | (uintptr_t)p.v_cache | (uintptr_t)p.q | (uintptr_t)p.part_o) & 15) == 0;
     if (int rc = launch_prefix_simple_rows<T>(p, false, prefix_rows, wide, stream)) return rc;
     if (int rc = launch_prefix_simple_rows<T>(p, true, own_rows, wide, stream)) return rc;
-    const long rows = (long)p.n_tokens * p.n_heads;
-    const cudaError_t e = launch_chained(prefix_merge_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, p);
+    const cudaError_t e = launch_chained(prefix_merge_kernel<T>, dim3(prefix_merge_blocks(p)), dim3(128), 0, stream, p);
     if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }

@@ -92,10 +92,14 @@ static int launch_copies(const CopyPools& pools, const CopyItem* items, int n, i
 
 using namespace mdma;
 
-// pools: n_pools x (address, bytes of a page, of a site, of a row, sites); rows: leading rows of each copy (null: page_rows).
-// `launches` gets the number of kernels.
-extern "C" int mdma_copy_pages(const long long* pool_words, int n_pools, int n_pages, int page_rows, const int* src, const int* dst,
-                               const int* rows, int n, int* launches, cudaStream_t stream) {
+// words: number of pools, pages, rows a page, copies, addresses of the lists (source pages, destination pages, leading rows of each
+// copy or null: whole pages), the number of launches (written here); then for every pool its address, bytes of a page, of a site
+// and of a row, and its sites.
+extern "C" int mdma_copy_pages(long long* words, cudaStream_t stream) {
+    const int n_pools = (int)words[0], n_pages = (int)words[1], page_rows = (int)words[2], n = (int)words[3];
+    const int *src = (const int*)(uintptr_t)words[4], *dst = (const int*)(uintptr_t)words[5], *rows = (const int*)(uintptr_t)words[6];
+    long long *launches = words + 7;
+    const long long* pool_words = words + 8;
     *launches = 0;
     MDMA_REQUIRE(n_pools > 0 && n_pages > 0 && page_rows > 0 && n >= 0, "copy_pages: %d pools of %d pages of %d rows", n_pools, n_pages, page_rows);
     if (n == 0) return 0;
@@ -132,8 +136,9 @@ extern "C" int mdma_copy_pages(const long long* pool_words, int n_pools, int n_p
         }
         const int vec = (align & 15) == 0 ? 16 : (align & 3) == 0 ? 4 : (align & 1) == 0 ? 2 : 1;
         for (int i = 0; i < kept && !rc;) {
-            const int take = kept - i <= 32 ? kept - i : kept - i < 1000 ? kept - i : 1000;
-            rc = take <= 32 ? launch_copies<32>(pools, items + i, take, vec, sms, stream) : launch_copies<1000>(pools, items + i, take, vec, sms, stream);
+            const int take = kept - i < 1000 ? kept - i : 1000;
+            rc = take <= 16 ? launch_copies<16>(pools, items + i, take, vec, sms, stream) : take <= 128 ? launch_copies<128>(pools, items + i, take, vec, sms, stream)
+                                                                                                : launch_copies<1000>(pools, items + i, take, vec, sms, stream);
             i += take;
             ++*launches;
         }

@@ -79,17 +79,17 @@ static inline long prefix_tiles_bound(const PrefixParams& p, int tile_tokens) {
     return (long)p.n_tokens / tile_tokens + p.n_groups;
 }
 
-// out[token, head] from its parts: those of its prefix in order, then those of its own keys.  One warp a row: a lane a part for the
-// maxima, the sums and the shares (at most 64 parts), then all lanes over the parts' numbers, eight parts in flight.
+// out[token, head] from its parts: those of its prefix in order, then those of its own keys.  One warp for 64 numbers of a row: a lane
+// a part for the maxima, the sums and the shares (at most 64 parts), then all lanes over the parts' numbers, eight parts in flight.
 template <typename T>
 __global__ void __launch_bounds__(128)
 prefix_merge_kernel(const PrefixParams p) {
     chain_release();
     chain_wait();
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);         // token * heads + head
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, D = p.head_dim, chunks = (D + 63) / 64;
+    const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 5), row = item / chunks;            // row: token * heads + head
     if (row >= (long)p.n_tokens * p.n_heads) return;
-    const int slots = p.pieces + p.own_splits, D = p.head_dim;
+    const int slots = p.pieces + p.own_splits;
     const int used = p.whole || p.pieces == 0 ? p.pieces : prefix_pieces_used(p.seq_skip[p.tok_seq[row / p.n_heads]], p.pieces, p.unit), parts = used + p.own_splits;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * slots;
     auto slot_of = [&](int s) { return s < used ? s : p.pieces + s - used; };
@@ -107,8 +107,8 @@ prefix_merge_kernel(const PrefixParams p) {
     if (p.sinks) l += exp2f(p.sinks[row % p.n_heads] * p.sink_rate - m);
     const float* o = p.part_o + row * slots * D;
     T* to = reinterpret_cast<T*>(p.out) + row * D;
-    for (int d0 = 0; d0 < D; d0 += 64) {             // two numbers a lane, 32 apart
-        const int d = d0 + lane;
+    {                                                // two numbers a lane, 32 apart
+        const int d = (int)(item % chunks) * 64 + lane;
         const bool one = d < D, two = d + 32 < D;
         float a0 = 0.f, a1 = 0.f;
         for (int s0 = 0; s0 < parts; s0 += 8) {
@@ -128,6 +128,10 @@ prefix_merge_kernel(const PrefixParams p) {
         if (one) to[d] = from_float<T>(a0 / l);
         if (two) to[d + 32] = from_float<T>(a1 / l);
     }
+}
+
+static inline unsigned prefix_merge_blocks(const PrefixParams& p) {
+    return (unsigned)(((long)p.n_tokens * p.n_heads * ((p.head_dim + 63) / 64) + 3) / 4);
 }
 
 // The arguments as one array of 64-bit words, in the order below (a step makes this call once a layer: converting thirty

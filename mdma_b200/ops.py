@@ -7,6 +7,7 @@ is no fallback: without the compiled library, or off the GPU, these raise.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 from typing import Optional
@@ -1115,7 +1116,7 @@ def matrix_memory_token(proj, cols, g_col: int, i_bias, f_bias, cap: float, q_sc
 # ---- pages of the cache, and attention of sequences that share their beginning ------------------------------------------------
 def _need_current(t: torch.Tensor) -> None:
     """A launch goes to a stream of the current device: tensors of another one are refused."""
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise KernelError(f"the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
@@ -1125,30 +1126,39 @@ def copy_pages(pools, src, dst, rows=None) -> None:
     group; heads, sizes and dtypes may differ).  `src`, `dst`, `rows`: numbers on the host; they travel with the launch, so
     nothing is uploaded and a captured launch keeps them.  A page may be copied to several others, but is not written twice
     and not both read and written in one call."""
-    pools = list(pools)
     if not pools:
         return
-    _need_cuda(*pools)
-    n_pages, page_size = pools[0].shape[1:3]
-    words = []
-    for p in pools:
-        if p.device != pools[0].device or p.dim() < 3 or p.shape[1:3] != (n_pages, page_size) or not p.is_contiguous():
-            raise KernelError("copy_pages takes contiguous pools [sites, pages, page_size, ...] of one device with the same "
-                              "pages and page size")
-        size = p.element_size()
-        words += (p.data_ptr(), p.stride(1) * size, p.stride(0) * size, p.stride(2) * size, p.shape[0])
-    _need_current(pools[0])
-    n = len(src)
+    n, n_pages = len(src), None
     if len(dst) != n or (rows is not None and len(rows) != n):
         raise KernelError(f"copy_pages: {n} pages to copy from, {len(dst)} to copy to, {n if rows is None else len(rows)} row counts")
-    if n == 0 or pools[0].numel() == 0:
+    # one array of 64-bit words takes all arguments: converting a dozen one by one costs more than the launch
+    words = array.array("q", (0, 0, 0, 0, 0, 0, 0, 0))
+    for p in pools:
+        if not p.is_cuda:
+            raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
+        stride, shape = p.stride(), p.shape
+        if n_pages is None and len(shape) >= 3:
+            n_pages, page_size, device = shape[1], shape[2], p.get_device()
+            _need_current(p)
+        if len(shape) < 3 or shape[1] != n_pages or shape[2] != page_size or p.get_device() != device or not p.is_contiguous():
+            raise KernelError("copy_pages takes contiguous pools [sites, pages, page_size, ...] of one device with the same "
+                              "pages and page size")
+        if p.numel() == 0:
+            return
+        size = p.element_size()
+        words.extend((p.data_ptr(), stride[1] * size, stride[0] * size, stride[2] * size, shape[0]))
+    if n == 0:
         return
-    ints = ctypes.c_int * n
-    launches = ctypes.c_int(0)
-    _call("core", "mdma_copy_pages", (ctypes.c_longlong * len(words))(*words), _i(len(pools)), _i(n_pages), _i(page_size),
-          ints(*src), ints(*dst), None if rows is None else ints(*rows), _i(n), ctypes.byref(launches), _stream(), launches=0)
+    try:
+        lists = [array.array("i", x) for x in ((src, dst) if rows is None else (src, dst, rows))]
+    except (OverflowError, TypeError) as e:
+        raise KernelError(f"copy_pages: {e}") from None
+    addresses = [x.buffer_info()[0] for x in lists]
+    words[0], words[1], words[2], words[3] = len(pools), n_pages, page_size, n
+    words[4], words[5], words[6] = addresses[0], addresses[1], addresses[2] if rows is not None else 0
+    _call("core", "mdma_copy_pages", ctypes.c_void_p(words.buffer_info()[0]), _stream(), launches=0)
     global LAUNCHES
-    LAUNCHES += launches.value
+    LAUNCHES += words[7]
 
 
 def copy_slots(states, src, dst) -> None:
@@ -1174,7 +1184,7 @@ def _prefix_rows(rows: int) -> int:
 
 def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int = 148) -> tuple[int, int]:
     """(pieces of a prefix, pieces of a sequence's own keys) of a step on the CUDA cores, 32 keys each at least, for about four
-    blocks an SM.  Of single tokens it follows from the most sequences the engine can hold, not from the live ones, so that a
+    blocks an SM (two of 64 rows, which is what its shared memory takes).  Of single tokens it follows from the most sequences the engine can hold, not from the live ones, so that a
     request's sums are cut at the same places when a batch mate ends."""
     one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
@@ -1182,8 +1192,9 @@ def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int = 148) -> tuple[
 
     def tiles(rows, of_tokens):                      # blocks of `rows` query rows over so many tokens, all kv heads
         return -(-of_tokens // max(1, rows // group)) * -(-group // rows) * n_kv_heads
-    pieces = 4 * sms // tiles(_prefix_rows(tokens * group), tokens)
-    own = 4 * sms // (tiles(_prefix_rows(ctx.max_new * group), ctx.max_new) * seqs)
+    rows, own_rows = _prefix_rows(tokens * group), _prefix_rows(ctx.max_new * group)
+    pieces = (2 if rows == 64 else 4) * sms // tiles(rows, tokens)
+    own = (2 if own_rows == 64 else 4) * sms // (tiles(own_rows, ctx.max_new) * seqs)
     return max(1, min(pieces, 32, -(-g.most_len // 32))), max(1, min(own, 32, -(-g.most_own // 32)))
 
 
@@ -1196,36 +1207,40 @@ def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int
                  sinks_log2: bool):
     """The arguments of the prefix attention kernels as one array (see csrc/prefix.cuh)."""
     g = ctx.prefix
-    words = (q.data_ptr(), q.stride(0), view.k.data_ptr(), view.v.data_ptr(), ctx.seq_start.data_ptr(), ctx.seq_pos0.data_ptr(),
-             ctx.seq_slot.data_ptr(), ctx.tok_seq.data_ptr(), view.page_table.data_ptr(), view.max_pages, view.page_size,
-             view.k.shape[0], g.group_len.data_ptr(), g.group_seq.data_ptr(), g.tok_first.data_ptr(), g.toks.data_ptr(),
-             g.seq_skip.data_ptr(), out.data_ptr(), scratch.data_ptr(), scratch.numel(), g.n_groups, ctx.n_seqs, ctx.n_tokens,
-             ctx.max_new, n_heads, n_kv_heads, head_dim, pieces, own_splits, 0 if sinks is None else sinks.data_ptr(),
-             0 if status is None else status.data_ptr(), int(sinks_log2))
-    return (ctypes.c_longlong * 32)(*words)
+    return array.array("q", (
+        q.data_ptr(), q.stride(0), view.k.data_ptr(), view.v.data_ptr(), ctx.seq_start.data_ptr(), ctx.seq_pos0.data_ptr(),
+        ctx.seq_slot.data_ptr(), ctx.tok_seq.data_ptr(), view.page_table.data_ptr(), view.max_pages, view.page_size,
+        view.k.size(0), g.group_len.data_ptr(), g.group_seq.data_ptr(), g.tok_first.data_ptr(), g.toks.data_ptr(),
+        g.seq_skip.data_ptr(), out.data_ptr(), scratch.data_ptr(), scratch.numel(), g.n_groups, ctx.n_seqs, ctx.n_tokens,
+        ctx.max_new, n_heads, n_kv_heads, head_dim, pieces, own_splits, 0 if sinks is None else sinks.data_ptr(),
+        0 if status is None else status.data_ptr(), int(sinks_log2)))
 
 
 def prefix_checks(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, sinks) -> None:
-    """What the prefix attention kernels cannot check of their arguments."""
-    g = ctx.prefix
-    ints = (ctx.seq_start, ctx.seq_pos0, ctx.seq_slot, ctx.tok_seq, view.page_table, g.group_len, g.group_seq, g.tok_first, g.toks,
-            g.seq_skip)
-    _need_cuda(q, view.k, view.v, out, sinks, *ints)
+    """What the prefix attention kernels cannot check of their arguments.  (In few calls: a step asks once a layer.)"""
+    g, k, v = ctx.prefix, view.k, view.v
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and out.is_cuda and (sinks is None or sinks.is_cuda)):
+        raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
     _need_current(q)
-    if any(t.dtype != torch.int32 for t in ints):
-        raise KernelError("positions, page tables and groups are int32")
-    if (view.k.dtype != q.dtype or view.v.dtype != q.dtype or out.dtype != q.dtype or q.dim() != 2 or q.stride(1) != 1
-            or not view.k.is_contiguous() or not view.v.is_contiguous() or not out.is_contiguous() or not view.page_table.is_contiguous()):
+    int32 = torch.int32
+    for t in (ctx.seq_start, ctx.seq_pos0, ctx.seq_slot, ctx.tok_seq, view.page_table, g.group_len, g.group_seq, g.tok_first, g.toks,
+              g.seq_skip):
+        if t.dtype is not int32 or not t.is_cuda:
+            raise KernelError("positions, page tables and groups are int32, on the device")
+    dtype, rows, shape = q.dtype, q.shape, out.shape
+    if (k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or len(rows) != 2 or q.stride(1) != 1
+            or not (k.is_contiguous() and v.is_contiguous() and out.is_contiguous() and view.page_table.is_contiguous())):
         raise KernelError("queries, caches and results have one dtype; caches and results are contiguous")
-    if (n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads or view.k.shape != view.v.shape
-            or tuple(view.k.shape[1:]) != (view.page_size, n_kv_heads, head_dim) or q.shape[0] < ctx.n_tokens
-            or q.shape[1] < n_heads * head_dim or out.shape[0] < ctx.n_tokens or out.shape[1] != n_heads * head_dim):
+    if (n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads or len(k.shape) != 4 or k.shape != v.shape
+            or k.size(1) != view.page_size or k.size(2) != n_kv_heads or k.size(3) != head_dim or len(shape) != 2
+            or rows[0] < ctx.n_tokens or rows[1] < n_heads * head_dim or shape[0] < ctx.n_tokens or shape[1] != n_heads * head_dim):
         raise KernelError(f"{n_heads} heads over {n_kv_heads} kv heads of {head_dim} do not fit queries {tuple(q.shape)}, caches "
-                          f"{tuple(view.k.shape)} and results {tuple(out.shape)}")
-    if (g.group_len.numel() < g.n_groups or g.group_seq.numel() < g.n_groups or g.tok_first.numel() < g.n_groups + 1
-            or g.toks.numel() < ctx.n_tokens or g.seq_skip.numel() < ctx.n_seqs):
-        raise KernelError("the groups' tables are shorter than the step")
-    if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != n_heads):
+                          f"{tuple(k.shape)} and results {tuple(out.shape)}")
+    if (g.group_len.numel() < g.n_groups or g.group_seq.numel() < g.n_groups or g.tok_first.numel() <= g.n_groups
+            or g.toks.numel() < ctx.n_tokens or g.seq_skip.numel() < ctx.n_seqs or ctx.seq_start.numel() <= ctx.n_seqs
+            or ctx.seq_pos0.numel() < ctx.n_seqs or ctx.seq_slot.numel() < ctx.n_seqs or ctx.tok_seq.numel() < ctx.n_tokens):
+        raise KernelError("the groups' or sequences' tables are shorter than the step")
+    if sinks is not None and (sinks.dtype is not torch.float32 or not sinks.is_contiguous() or sinks.numel() != n_heads):
         raise KernelError("sinks are one float a head")
 
 
@@ -1249,5 +1264,5 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
         raise KernelError(f"prefix attention needs {need} floats of scratch, {scratch.numel()} given")
     words = prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sinks, None, False)
     group = n_heads // n_kv_heads
-    _call("core", "mdma_prefix_attention_simple", words, _i(32), _f(scale), _i(dtype_code(q.dtype)),
+    _call("core", "mdma_prefix_attention_simple", ctypes.c_void_p(words.buffer_info()[0]), _i(32), _f(scale), _i(dtype_code(q.dtype)),
           _i(_prefix_rows(ctx.n_tokens * group)), _i(_prefix_rows(ctx.max_new * group)), _stream(), launches=3)

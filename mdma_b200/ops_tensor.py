@@ -702,7 +702,7 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
         st.need(need, "attention over shared prefixes")
         scratch = st.scratch
     else:
-        scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else out        # (nothing is kept there)
     words = ops.prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sink_log2, st.status, True)
-    _call("tensor", "mdma_prefix_attention", words, _i(32), _f(scale), _i(kind), _stream(),
+    _call("tensor", "mdma_prefix_attention", ctypes.c_void_p(words.buffer_info()[0]), _i(32), _f(scale), _i(kind), _stream(),
           launches=(pieces > 0) + (own > 0) + (pieces > 1 if own == 0 else own > 1 or ctx.max_new > 1 or n_heads // n_kv_heads > 16 or view.page_size % 32 != 0))
