@@ -233,9 +233,10 @@ static int launch_prefix_stream(const PrefixParams& p, int sms, cudaStream_t str
     };
     // as many warps a block as leave every block resident at once, two at least (51 sequences x 32 kv heads, own keys and prefixes:
     // 53 us in rounds of two-warp blocks, 56 with one warp, 67 with four)
-    const int nw = blocks <= sms ? 12 : blocks <= 3l * sms ? 4 : 2;
+    const int nw = blocks <= sms ? 12 : blocks <= 3l * sms ? 4 : blocks <= 4l * sms ? 3 : 2;
 #define MDMA_STREAM(DM, KB) (nw == 12 ? run(prefix_stream_kernel<DM, KB, 12, SHARED>, 12, PoSmem<DM, KB, 12>::kBytes) \
                            : nw == 4 ? run(prefix_stream_kernel<DM, KB, 4, SHARED>, 4, PoSmem<DM, KB, 4>::kBytes) \
+                           : nw == 3 ? run(prefix_stream_kernel<DM, KB, 3, SHARED>, 3, PoSmem<DM, KB, 3>::kBytes) \
                                      : run(prefix_stream_kernel<DM, KB, 2, SHARED>, 2, PoSmem<DM, KB, 2>::kBytes))
     return kb == 64 ? MDMA_STREAM(64, 64) : p.head_dim <= 64 ? MDMA_STREAM(64, 32) : MDMA_STREAM(128, 32);
 #undef MDMA_STREAM

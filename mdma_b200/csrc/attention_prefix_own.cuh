@@ -27,7 +27,7 @@ struct PoSmem {
 };
 
 template <int DMAX, int KB, int NW, bool SHARED>
-__global__ void __launch_bounds__(NW * 32, NW >= 8 ? 1 : NW == 4 ? 3 : 5)
+__global__ void __launch_bounds__(NW * 32, NW >= 8 ? 1 : NW == 4 ? 3 : NW == 3 ? 4 : 5)
 prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams p) {
     using L = PoSmem<DMAX, KB, NW>;
     constexpr int kChunks = DMAX / 8, kHalf = KB * 128;
