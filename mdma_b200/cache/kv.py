@@ -249,6 +249,8 @@ class SequenceCache:
             if g.need.bounded and any(p not in have for p in range(g.need.first_key(length) // self.page_size, last + 1)):
                 return ValueError("a windowed group has already released pages of the shared part")
             want = n if length % self.page_size and last in have else 0
+            if want and g.k is not None and not g.k.is_cuda:
+                return ValueError("pages are copied on the GPU only: this cache lies elsewhere")
             if want > g.pages.free_count:
                 return CacheFull(f"{want} more cache pages of {self.page_size} tokens are wanted, {g.pages.free_count} of "
                                  f"{g.n_pages} are free")
@@ -405,6 +407,8 @@ class SequenceCache:
         rows = length % self.page_size
         own = [g for g in self.groups if rows and g.seq_pages.get(slot, {}).get(last) in g.holders]
         for g in own:
+            if g.k is not None and not g.k.is_cuda:
+                raise ValueError("pages are copied on the GPU only: this cache lies elsewhere")
             if g.pages.free_count + sum(1 for p, page in g.seq_pages[slot].items() if p > last and page not in g.holders) < 1:
                 raise CacheFull(f"a page for the kept rows of a shared one is wanted, none of {g.n_pages} is free")
         for g in self.groups:

@@ -326,18 +326,6 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (ra >= rb) continue;
             const int end = w.s.key1 - w.key, steps = w.steps();                     // block rows beyond `end` belong to nobody
             const bool shared = w.seg == 0 && len > 0;
-            if (end < steps * 64) {
-                // such value rows are cleared before the product reads them: a weight of zero times what is not finite would not be
-                // zero (each tile clears them for its own product; the other may be behind)
-                const int s = j & 1;
-                ok = __all_sync(0xffffffffu, ptx::mbar_wait(v_full(s), (j >> 1) & 1, abort_flag));
-                if (!ok) break;
-                for (int e = threadIdx.x & 127; e < halves * kPtKeys * 8; e += 128) {
-                    const int h = e / (kPtKeys * 8), kr = (e >> 3) % kPtKeys, c = e & 7;
-                    if (kr >= end) *reinterpret_cast<uint4*>(smem + kPtSmemV + s * kPtSlot + h * kPtHalf + kr * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                ptx::fence_proxy_async_shared();
-            }
             int c0 = 0, c1 = end;                                // columns of the block that this row sees
             if (!shared) {
                 c0 = w.s.key0 - w.key;
@@ -349,6 +337,19 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (!ok) break;
             ptx::tc_fence_after_sync();
             ++seen;
+            if (end < steps * 64) {
+                // such value rows are cleared before the product reads them: a weight of zero times what is not finite would not be
+                // zero (each tile clears them for its own product, the other may be behind; and only now that its scores are
+                // there: a tile that many blocks do not concern would otherwise take an earlier block's values for this one's)
+                const int s = j & 1;
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(v_full(s), (j >> 1) & 1, abort_flag));
+                if (!ok) break;
+                for (int e = threadIdx.x & 127; e < halves * kPtKeys * 8; e += 128) {
+                    const int h = e / (kPtKeys * 8), kr = (e >> 3) % kPtKeys, c = e & 7;
+                    if (kr >= end) *reinterpret_cast<uint4*>(smem + kPtSmemV + s * kPtSlot + h * kPtHalf + kr * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                ptx::fence_proxy_async_shared();
+            }
             // twice over the row, 64 keys at a time (as straight code with the whole row in registers it spilled and was 2% slower)
             float2 sum = make_float2(0.f, 0.f), sum2 = make_float2(0.f, 0.f);
             float2 off = make_float2(0.f, 0.f);

@@ -1136,25 +1136,25 @@ def copy_pages(pools, src, dst, rows=None) -> None:
     for p in pools:
         if not p.is_cuda:
             raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
-        stride, shape = p.stride(), p.shape
+        shape = p.shape
         if n_pages is None and len(shape) >= 3:
             n_pages, page_size, device = shape[1], shape[2], p.get_device()
             _need_current(p)
         if len(shape) < 3 or shape[1] != n_pages or shape[2] != page_size or p.get_device() != device or not p.is_contiguous():
             raise KernelError("copy_pages takes contiguous pools [sites, pages, page_size, ...] of one device with the same "
                               "pages and page size")
-        if p.numel() == 0:
-            return
-        size = p.element_size()
-        words.extend((p.data_ptr(), stride[1] * size, stride[0] * size, stride[2] * size, shape[0]))
-    if n == 0:
+        total = p.numel() * p.element_size()         # (the strides of a dimension of one element say nothing)
+        if total:
+            site = total // shape[0]
+            words.extend((p.data_ptr(), site // n_pages, site, site // (n_pages * page_size), shape[0]))
+    if n == 0 or len(words) == 8:
         return
     try:
         lists = [array.array("i", x) for x in ((src, dst) if rows is None else (src, dst, rows))]
     except (OverflowError, TypeError) as e:
         raise KernelError(f"copy_pages: {e}") from None
     addresses = [x.buffer_info()[0] for x in lists]
-    words[0], words[1], words[2], words[3] = len(pools), n_pages, page_size, n
+    words[0], words[1], words[2], words[3] = (len(words) - 8) // 5, n_pages, page_size, n
     words[4], words[5], words[6] = addresses[0], addresses[1], addresses[2] if rows is not None else 0
     _call("core", "mdma_copy_pages", ctypes.c_void_p(words.buffer_info()[0]), _stream(), launches=0)
     global LAUNCHES
@@ -1219,14 +1219,17 @@ def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int
 def prefix_checks(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, sinks) -> None:
     """What the prefix attention kernels cannot check of their arguments.  (In few calls: a step asks once a layer.)"""
     g, k, v = ctx.prefix, view.k, view.v
-    if not (q.is_cuda and k.is_cuda and v.is_cuda and out.is_cuda and (sinks is None or sinks.is_cuda)):
+    device, int32 = q.get_device(), torch.int32
+    if device < 0:
         raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
     _need_current(q)
-    int32 = torch.int32
+    if (k.get_device() != device or v.get_device() != device or out.get_device() != device
+            or (sinks is not None and sinks.get_device() != device)):
+        raise KernelError("queries, caches, results and sinks are on one device")
     for t in (ctx.seq_start, ctx.seq_pos0, ctx.seq_slot, ctx.tok_seq, view.page_table, g.group_len, g.group_seq, g.tok_first, g.toks,
               g.seq_skip):
-        if t.dtype is not int32 or not t.is_cuda:
-            raise KernelError("positions, page tables and groups are int32, on the device")
+        if t.dtype is not int32 or t.get_device() != device:
+            raise KernelError("positions, page tables and groups are int32, on the queries' device")
     dtype, rows, shape = q.dtype, q.shape, out.shape
     if (k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or len(rows) != 2 or q.stride(1) != 1
             or not (k.is_contiguous() and v.is_contiguous() and out.is_contiguous() and view.page_table.is_contiguous())):
@@ -1260,8 +1263,8 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     need = prefix_scratch_floats(ctx.n_tokens, n_heads, pieces + own, head_dim)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-    elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need:
-        raise KernelError(f"prefix attention needs {need} floats of scratch, {scratch.numel()} given")
+    elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.get_device() != q.get_device():
+        raise KernelError(f"prefix attention needs {need} floats of scratch on the queries' device, {scratch.numel()} given")
     words = prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sinks, None, False)
     group = n_heads // n_kv_heads
     _call("core", "mdma_prefix_attention_simple", ctypes.c_void_p(words.buffer_info()[0]), _i(32), _f(scale), _i(dtype_code(q.dtype)),

@@ -196,7 +196,8 @@ def expect(before, src, dst, rows):
 
 
 def same(a, b):
-    return torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    raw = lambda t: torch.empty(t.shape, dtype=t.dtype).copy_(t).flatten().view(torch.uint8)  # noqa: E731
+    return torch.equal(raw(a), raw(b))
 
 
 @pytest.mark.gpu
@@ -244,6 +245,30 @@ def test_copies_into_a_view_of_wider_memory():
     assert torch.equal(p.cpu(), want) and torch.equal(rest, whole[3 + p.numel():])
 
 
+def test_a_cache_off_the_gpu_does_not_fork_inside_a_page():
+    c = SequenceCache([KVNeed(2, 16)], [None], 64 * 8, 4, 256, torch.float32, "cpu", 64)
+    a = c.acquire()
+    grow(c, a, 70)
+    with pytest.raises(ValueError, match="GPU"):
+        c.fork(a)
+    c.check()
+    (b,) = c.fork(a, 1, 64)
+    with pytest.raises(ValueError, match="GPU"):
+        c.truncate(b, 10)
+    c.check()
+    assert c.length(a) == 70 and c.length(b) == 64
+
+
+@pytest.mark.gpu
+def test_pools_of_nothing_and_pages_of_one_row():
+    a, b = pool((2, 6, 1, 3), torch.float32, 0), pool((1, 6, 1, 1), torch.bfloat16, 1)
+    on = [torch.empty(0, 6, 1, 4, device="cuda"), a.cuda(), torch.empty(2, 6, 1, 0, device="cuda"), b.cuda().as_strided((1, 6, 1, 1), (99, 1, 77, 5))]
+    ops.copy_pages(on, [2, 2, 5], [0, 1, 3], [1, 0, 1])
+    want = [expect(x, [2, 5], [0, 3], None) for x in (a, b)]
+    assert same(on[1].cpu(), want[0]) and same(on[3].cpu(), want[1])
+    ops.copy_pages(on[:1], [2], [0])
+
+
 @pytest.mark.gpu
 def test_copies_refuse_and_leave_the_pools():
     p = pool((2, 6, 8, 3), torch.float32, 0).cuda()
@@ -256,6 +281,9 @@ def test_copies_refuse_and_leave_the_pools():
         ops.copy_pages([p, p[:, :5].contiguous()], [0], [1])
     with pytest.raises(KernelError):
         ops.copy_pages([p.transpose(0, 1)], [0], [1])
+    for src in ([2 ** 40], [0.5], ["a"]):
+        with pytest.raises(KernelError):
+            ops.copy_pages([p], src, [1])
     assert same(p, before)
     ops.copy_pages([], [0], [1])
 

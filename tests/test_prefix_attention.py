@@ -109,6 +109,83 @@ def test_as_if_nothing_were_shared(path):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news", [1, 5], ids=["single tokens", "prompts"])
+@pytest.mark.parametrize("path", ["float32", "bfloat16", "tensor"])
+@pytest.mark.parametrize("geometry", [(8, 2, 64, 64), (4, 4, 128, 16), (4, 1, 32, 32)], ids=str)
+def test_what_is_not_finite_stays_with_its_sequence(geometry, path, news):
+    """A sequence whose own keys and values hold infinities and NaN gets what its formula gives; the others do not notice."""
+    heads, kv_heads, dim, ps = geometry
+    dtype = torch.float32 if path == "float32" else torch.bfloat16
+    ctx, q, view, dense = make_batch([(130, [(9, news), (0, news), (70, news), (3, news)])], heads, kv_heads, dim, ps, dtype, 5, DEV)
+    bad = 2
+    pos = int(ctx.seq_pos0[bad])
+    page = int(view.page_table[ctx.seq_slot[bad], pos // ps])
+    view.k[page, pos % ps] = float("nan")
+    view.v[page, pos % ps] = float("inf")
+    out = torch.empty(ctx.n_tokens, heads * dim, dtype=dtype, device=DEV)
+    (ops_tensor if path == "tensor" else ops).prefix_attention(ctx, q, view, out, heads, kv_heads, dim, scale_of(dim))
+    want, size, spread, keys = definition(ctx, q, dense, heads, kv_heads, dim, scale_of(dim))
+    keep = torch.tensor([s != bad for s in ctx.tok_seq.tolist()])
+    check_close(out.cpu()[keep], (want[keep], size[keep], spread[keep], keys[keep]), dim, dtype)
+    a = int(ctx.seq_start[bad])
+    assert not torch.isfinite(out[a]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", ["float32", "tensor"])
+def test_captured_on_another_stream_and_replayed(path):
+    """A captured call takes what lies in its tensors at every replay; calls on two streams do not share their parts."""
+    dtype = torch.float32 if path == "float32" else torch.bfloat16
+    fn = ops.prefix_attention if path == "float32" else ops_tensor.prefix_attention
+    cases = [make_batch([(900, [(i, 1) for i in range(20)])], 8, 2, 64, 64, dtype, seed, DEV) for seed in (1, 2)]
+    outs = [torch.empty(20, 512, dtype=dtype, device=DEV) for _ in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        for (ctx, q, view, _), out, stream in zip(cases, outs, streams):
+            with torch.cuda.stream(stream):
+                fn(ctx, q, view, out, 8, 2, 64, 0.125)
+    torch.cuda.synchronize()
+    for (ctx, q, view, dense), out in zip(cases, outs):
+        check_close(out, definition(ctx, q, dense, 8, 2, 64, 0.125), 64, dtype)
+    ctx, q, view, dense = cases[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fn(ctx, q, view, outs[0], 8, 2, 64, 0.125)
+    q2 = (torch.randn(q.shape, generator=torch.Generator().manual_seed(9)).to(dtype)).to(DEV)
+    q.copy_(q2)
+    outs[0].zero_()
+    graph.replay()
+    check_close(outs[0], definition(ctx, q2, dense, 8, 2, 64, 0.125), 64, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("plan", [(0, 1, 1), (0, 3, 1), (1, 1, 1), (5, 2, 1), (32, 1, 1), (1, 1, 0), (7, 1, 0), (9, 4, 0), (32, 16, 0), (3, 2, 2), (32, 32, 2)], ids=str)
+@pytest.mark.parametrize("geometry", [(8, 2, 64, 64), (32, 2, 128, 64), (3, 1, 96, 128)], ids=str)
+def test_every_kernel_and_cut_of_single_tokens(geometry, plan, monkeypatch):
+    """Whichever kernel does the prefixes and into however many pieces the keys are cut."""
+    monkeypatch.setattr(ops_tensor, "prefix_plan", lambda *a: plan)
+    run_case([(1000, ONE), (0, [(300, 1)]), (65, [(0, 1)] * 7)], *geometry, torch.bfloat16, False, sink=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pieces", [1, 2, 5, 32])
+def test_every_cut_of_whole_lists(pieces, monkeypatch):
+    monkeypatch.setattr(ops_tensor, "prefix_plan", lambda *a: (pieces, 0, 0))
+    for name in ("prompts and single tokens", "prompts longer than the prefix", "groups and loners"):
+        run_case(dict(BATCHES)[name], 8, 2, 64, 64, torch.bfloat16, False, sink=pieces > 1)
+    run_case([(300, [(i % 3, 1 + i % 2) for i in range(200)])], 2, 2, 64, 64, torch.bfloat16, False)       # many sequences a block
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("plan", [(1, 1), (32, 32), (3, 2)], ids=str)
+def test_every_cut_on_the_cuda_cores(plan, monkeypatch):
+    monkeypatch.setattr(ops, "prefix_plan", lambda *a: plan)
+    for name in ("groups and loners", "prompts and single tokens"):
+        run_case(dict(BATCHES)[name], 6, 2, 72, 16, torch.float32, True, sink=True)
+
+
+@pytest.mark.gpu
 def test_refusals():
     ctx, q, view, _ = make_batch([(100, ONE)], 8, 2, 64, 64, torch.bfloat16, 0, DEV)
     out = torch.empty(ctx.n_tokens, 512, dtype=q.dtype, device=DEV)
