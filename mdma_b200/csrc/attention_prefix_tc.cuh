@@ -12,16 +12,22 @@
 // tile's P V and its next S one behind the other, so whoever sees S(j) complete knows that P(j-1) V(j-1) is, too, and the
 // tiles' S are complete half a period apart.
 // The weights are taken against a reference that moves only when a row's maximum has grown by more than 2^8 since; O is
-// rescaled only then.  Of every four exponentials one goes through a polynomial on the multiply-add units (`exp2_poly`), which
-// the exponential unit (16 results a cycle and SM) would be the bound of otherwise.
-// Measured, cycles a block of 128 keys and both tiles (the tensor pipe's own: 2,048): 3,400.  What was slower: two threads a row
-// (the issue slots of sixteen softmax warps are the bound then) 4,200; a warp that issues for each tile, both in step, 4,850; P V
-// behind the whole softmax 3,450; steps of 64 keys with two places for S (products of N = 64 cost as much as of N = 128) 3,700.
-// 8,960 rows a kv head over 8,000 keys, 32 heads of 128: 321 us, 996 TFLOP/s.
+// rescaled only then.
+// Measured, cycles a block of 128 keys and both tiles (the tensor pipe's own: 2,048; the exponential unit's as many): 3,400,
+// of which a tile's softmax and its products, one behind the other, are the chain.  What was slower or no faster: two threads a
+// row (the issue slots of sixteen softmax warps are the bound then) 4,200; a warp that issues for each tile, both in step, 4,850;
+// P V behind the whole softmax 3,450; steps of 64 keys with two places for S (products of N = 64 cost as much as of N = 128)
+// 3,700; the first half's weights before the row's maximum is known 3,450; a quarter of the exponentials by a polynomial on the
+// multiply-add units 3,400; the next blocks asked into L2 ahead, 15% more where they come from memory.
+// 8,960 rows a kv head over 8,000 keys, 32 heads of 128: 320 us, 1.0 PFLOP/s.
 //
 // The list: the prefix's blocks, which all rows see, and (`whole`) behind them the own blocks of every sequence with tokens in the
 // tiles, which only that sequence's rows see: the others' lanes of O are left out of the product, so that what they are
 // multiplied with does not reach them.  `pieces` blocks share a list; each then leaves its sums for the merge.
+//
+// The kernel takes all 512 columns of tensor memory and is launched programmatically, which is sound in the order that it
+// keeps: it waits for the kernel before it, takes the columns, and only then lets the next one start.  So no block waits for columns
+// beside a block that waits for it, and a block needs no other one to be placed.
 #pragma once
 #include "prefix.cuh"
 #include "ptx.cuh"
@@ -69,8 +75,7 @@ struct PtWalk {
     __device__ __forceinline__ int steps() const { return s.key1 - key > 64 ? 2 : 1; }        // of 64 keys
 };
 
-// 2^x for x <= 126 by range reduction to [-1/2, 1/2] and a polynomial (minimax in the relative error, 2.7e-6; own fit); two at
-// once.  The sum with 1.5 2^23 leaves the nearest integer in the low bits, which move into the exponent.
+// Two products and sums, two sums at once.
 __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
     float2 d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
@@ -83,19 +88,6 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    const float magic = 12582912.0f;
-    x.x = fmaxf(x.x, -126.0f); x.y = fmaxf(x.y, -126.0f);
-    const float2 t = add_pair(x, make_float2(magic, magic));
-    const float2 n = add_pair(t, make_float2(-magic, -magic));
-    const float2 f = fma_pair(n, make_float2(-1.f, -1.f), x);
-    float2 y = fma_pair(f, make_float2(0.009570102207362652f, 0.009570102207362652f), make_float2(0.05591785907745361f, 0.05591785907745361f));
-    y = fma_pair(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
-    y = fma_pair(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-    y = fma_pair(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
-}
-
 __global__ void __launch_bounds__(kPtThreads, 1)
 prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -413,7 +405,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const float2 x = fma_pair(make_float2(sv[u * 32 + 2 * i], sv[u * 32 + 2 * i + 1]), rate, off);
-                            const float2 e = (i & 3) == 3 ? exp2_poly(x) : make_float2(ptx::ex2_approx(x.x), ptx::ex2_approx(x.y));
+                            const float2 e = make_float2(ptx::ex2_approx(x.x), ptx::ex2_approx(x.y));
                             if (i & 1) sum = add_pair(sum, e); else sum2 = add_pair(sum2, e);
                             const __nv_bfloat162 b2 = __floats2bfloat162_rn(e.x, e.y);
                             pk[i] = *reinterpret_cast<const uint32_t*>(&b2);

@@ -284,12 +284,6 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Writes 8 consecutive float columns of this thread's TMEM lane; pair with tmem_store_wait().
-__device__ __forceinline__ void tmem_store_8_nowait(uint32_t taddr, const float* v) {
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
 // Writes 16 consecutive 32-bit columns of this thread's TMEM lane; pair with tmem_store_wait().
 __device__ __forceinline__ void tmem_store_16_nowait(uint32_t taddr, const uint32_t* r) {
     asm volatile(
