@@ -136,8 +136,8 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
 
 
 def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_context: int, page_size: int) -> int:
-    """Scratch for single-token steps over shared prefixes: the parts of every sequence's softmaxes (steps of several tokens
-    use it as far as it goes)."""
+    """Scratch for single-token steps over shared prefixes: the parts of every sequence's softmaxes, of 512 sequences at most
+    (steps of more tokens use it as far as it goes; those that it does not hold read sequence by sequence)."""
     from types import SimpleNamespace
 
     from .. import ops, ops_tensor
@@ -149,7 +149,7 @@ def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_cont
             parts = sum(ops.prefix_plan(ctx, most, heads, kv_heads))
             if dtype == torch.bfloat16 and ops_tensor.attention_supported(heads, kv_heads, head_dim):
                 parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, head_dim, sms, page_size)[:2]))
-            need = max(need, ops.prefix_scratch_floats(max_slots, heads, parts, head_dim))
+            need = max(need, ops.prefix_scratch_floats(min(max_slots, 512), heads, parts, head_dim))
     return need
 
 
