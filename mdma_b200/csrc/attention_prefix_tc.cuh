@@ -285,17 +285,22 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const bool row_valid = r / G < tt && tok < count;
         const int token = row_valid ? p.toks[tile.first + tok] : -1;
         if (t == 0 || count > tt) {
-            // the row's query into shared memory, 128-byte rows with the 128-byte swizzle, zeros beyond the tile's rows (a row a
-            // thread, all of it in flight: with the rows' chunks dealt out over the threads, each asking for its row's token first, it
-            // took 3 to 9 us)
-            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (size_t)max(token, 0) * p.q_stride + (size_t)(kvh * G + r % G) * D;
+            // the warp's queries into shared memory, 128-byte rows with the 128-byte swizzle, zeros beyond the tile's rows: half a
+            // warp a row, all of it in flight (each lane has asked for its own row's token before)
+            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q);
+            const int c = lane & 15;
             uint4 x[16];
 #pragma unroll
-            for (int c = 0; c < 16; ++c)
-                x[c] = row_valid && c * 8 < D ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < 16; ++i) {
+                const int from = 2 * i + (lane >> 4), of = __shfl_sync(0xffffffffu, token, from);
+                x[i] = of >= 0 && c * 8 < D ? *reinterpret_cast<const uint4*>(q + (size_t)of * p.q_stride + (size_t)(kvh * G + (quad * 32 + from) % G) * D + c * 8)
+                                            : make_uint4(0u, 0u, 0u, 0u);
+            }
 #pragma unroll
-            for (int c = 0; c < 16; ++c)
-                if (c < halves * 8) *reinterpret_cast<uint4*>(smem + t * kPtSlot + (c >> 3) * kPtHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[c];
+            for (int i = 0; i < 16; ++i) {
+                const int to = quad * 32 + 2 * i + (lane >> 4);
+                if (c < halves * 8) *reinterpret_cast<uint4*>(smem + t * kPtSlot + (c >> 3) * kPtHalf + to * 128 + (((c & 7) ^ (to & 7)) << 4)) = x[i];
+            }
             ptx::fence_proxy_async_shared();
         }
         ptx::mbar_arrive(q_full);
