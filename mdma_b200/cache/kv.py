@@ -187,6 +187,7 @@ class SequenceCache:
         self.slots = FreeList(max_slots, "sequence slot")
         self.lengths: dict[int, int] = {}
         self.shares: dict[int, tuple[int, int]] = {}        # slot -> (number of its fork, tokens that the fork's sequences share)
+        self.families: dict[int, int] = {}                  # number of a fork -> the most sequences that have shared it at a time
         self._forks = 0
         self.groups: list[CacheGroup] = []
         self.site_group: dict[int, tuple[int, int]] = {}
@@ -228,7 +229,7 @@ class SequenceCache:
         self.slots.release(slot)
         for g in self.groups:
             g.release(slot)
-        self.shares.pop(slot, None)
+        self._share(slot, None)
         del self.lengths[slot]
 
     def _fork_refusal(self, slot: int, n: int, length: Optional[int]) -> Optional[Exception]:
@@ -255,6 +256,14 @@ class SequenceCache:
                 return CacheFull(f"{want} more cache pages of {self.page_size} tokens are wanted, {g.pages.free_count} of "
                                  f"{g.n_pages} are free")
         return None
+
+    def _share(self, slot: int, share: Optional[tuple[int, int]]) -> None:
+        """The sequence in `slot` shares this from now on (None: nothing)."""
+        old = self.shares.pop(slot, None)
+        if share is not None:
+            self.shares[slot] = share
+        if old is not None and old[0] in self.families and all(s[0] != old[0] for s in self.shares.values()):
+            del self.families[old[0]]                       # nobody is left of that fork
 
     def can_fork(self, slot: int, n: int = 1, length: Optional[int] = None) -> Optional[str]:
         """None if the sequence in `slot` can fork into `n` further ones, else the reason."""
@@ -295,9 +304,11 @@ class SequenceCache:
         if length:
             if self.shares.get(slot, (0, 0))[1] != length:
                 self._forks += 1
-                self.shares[slot] = (self._forks, length)
+                self._share(slot, (self._forks, length))
             for s in new:
-                self.shares[s] = self.shares[slot]
+                self._share(s, self.shares[slot])
+            fork = self.shares[slot][0]
+            self.families[fork] = max(self.families.get(fork, 0), sum(1 for s in self.shares.values() if s[0] == fork))
         return new
 
     def shared_prefixes(self, slots) -> list[tuple[int, list[int]]]:
@@ -309,6 +320,10 @@ class SequenceCache:
             if share is not None:
                 found.setdefault(share[0], (share[1], []))[1].append(i)
         return [found[f] for f in sorted(found)]
+
+    def most_members(self, slots) -> int:
+        """The most sequences that have shared a fork of one of these at a time (who has ended counts on while another is left)."""
+        return max((self.families[self.shares[s][0]] for s in slots if s in self.shares), default=0)
 
     def compact(self) -> int:
         """Move held pages from the rear of each group's pool to free ones at its front, so that the held pages are the pool's
@@ -422,7 +437,7 @@ class SequenceCache:
                 g.place(slot, last, page)
                 g.sync_tables()
         if self.shares.get(slot, (0, 0))[1] > length:
-            del self.shares[slot]                   # it has less than its fork shares
+            self._share(slot, None)                 # it has less than its fork shares
         self.lengths[slot] = length
 
     def view(self, site: int, state_site: Optional[int] = None) -> KVView:

@@ -32,6 +32,8 @@ BUCKET = 1024          # graphs are captured per this many positions of the long
 
 
 class DecodeSession:
+    most_prefix_graphs = 64         # of steps over shared prefixes
+
     def __init__(self, engine):
         self.engine, self.sampler = engine, engine.sampler
         self.params = SamplingParams.greedy()
@@ -159,7 +161,7 @@ class DecodeSession:
             if use_graph and self.graph_safe:
                 key = (B, self._bucket, draws)
                 if self.prefix is not None:       # what the grids and the tables' places follow from
-                    key += (self.prefix.n_groups, self.prefix.most_len, self.prefix.least_skip)
+                    key += (self.prefix.n_groups, self.prefix.most_len, self.prefix.least_skip, self.prefix.n_shared, self.prefix.most_members)
                 g = self.graphs.get(key)
                 if g is None:
                     # The first step at this batch size runs eagerly (it loads kernels); the same
@@ -181,7 +183,10 @@ class DecodeSession:
                         if was_enabled:
                             gc.enable()
                     self.graphs[key] = g
+                    self._drop_graphs()
                 else:
+                    if len(key) > 3:              # the last of them in the order of use
+                        self.graphs[key] = self.graphs.pop(key)
                     g.replay()
             else:
                 self._body(B, draws)
@@ -193,6 +198,14 @@ class DecodeSession:
             self._ring_base += self._kept - self.max_run
             self._kept = self.max_run
         return n
+
+    def _drop_graphs(self) -> None:
+        """Of the graphs of steps over shared prefixes the `most_prefix_graphs` used last are kept (their number has no bound of its own)."""
+        those = [key for key in self.graphs if len(key) > 3]
+        if len(those) > self.most_prefix_graphs:
+            torch.cuda.current_stream().synchronize()         # none of them is running
+            for key in those[:-self.most_prefix_graphs]:
+                del self.graphs[key]
 
     def read(self) -> list[tuple[list[int], list[int]]]:
         """The tokens and non-finite flags of every step since the last read, oldest first

@@ -142,13 +142,17 @@ def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_cont
 
     from .. import ops, ops_tensor
     ctx = SimpleNamespace(max_new=1, n_seqs=max_slots, n_tokens=max_slots, most_seqs=max_slots)
-    most = SimpleNamespace(most_len=max_context, most_own=max_context, most_tokens=max_slots, n_groups=1)
+    most = SimpleNamespace(most_len=max_context, most_own=max_context, most_tokens=max_slots, n_groups=1, n_shared=1)
     need = 0
     for part in model.all_parts():
         for heads, kv_heads, head_dim in getattr(part, "prefix_shapes", list)():
             parts = sum(ops.prefix_plan(ctx, most, heads, kv_heads))
             if dtype == torch.bfloat16 and ops_tensor.attention_supported(heads, kv_heads, head_dim):
-                parts = max(parts, sum(ops_tensor.prefix_plan(ctx, most, heads, kv_heads, head_dim, sms, page_size)[:2]))
+                for most.most_members in (1, max_slots):       # (fewer families or more: at most `prefix_tc_pieces`)
+                    pieces, own, kind = ops_tensor.prefix_plan(ctx, most, heads, kv_heads, head_dim, sms, page_size)
+                    if kind == ops_tensor.PREFIX_TC:
+                        pieces = ops_tensor.prefix_tc_pieces(max_slots, heads // kv_heads, kv_heads, sms)
+                    parts = max(parts, pieces + own)
             need = max(need, ops.prefix_scratch_floats(min(max_slots, 512), heads, parts, head_dim))
     return need
 
@@ -429,6 +433,7 @@ class Engine:
             up = lambda n: min(self.max_context, -(-n // 1024) * 1024)  # noqa: E731
             groups.most_len, groups.least_skip = up(groups.most_len), groups.least_skip // 1024 * 1024
             groups.most_own = up(max(pos0) + 1) - groups.least_skip
+            groups.most_members = self.cache.most_members([slots[m] for _, members in shared for m in members])
         return groups
 
     # ---- the step ----------------------------------------------------------

@@ -602,7 +602,6 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
     assert view.k.shape[-2:] == (n_kv_heads * maps, dim) and view.v.shape[-2:] == (n_kv_heads, v_dim)
     for t in (sink_log2, slope_log2):
         assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n_heads)
-    own_st = st
     st = st or _device_state(q.device)
     flush_pending(q.device, st)
     group = n_heads // n_kv_heads
@@ -638,8 +637,14 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
 
 
 # ---- attention of sequences that share their beginning (csrc/attention_prefix.cu) ------------------------------------------
+# Prefix bytes times sequences up to which every sequence of a single-token step reads its prefix by itself, and the query rows
+# of a kv head in the largest family up to which prefixes are streamed.  us, alone / streamed / tcgen05, heads of 128:
+# 4 sequences behind 300 tokens, 32/8 heads of 64: 5.5 / 11; 8 behind 2,048, 32/8 (64 MiB, 32 rows): 16.1 / 14.5 / 18.0;
+# 16 behind 2,048, 32/8 (128 MiB, 64 rows): 20.9 / 18.7 / 18.7; 16 behind 2,048, 32/32 (16 rows): 69 / 25.5 / 29.9;
+# 4 families of 6 behind 2,000, 32/8 (24 rows): - / 20.4 / 24.0; 6 of 8 behind 6,000, 32/8 (32 rows): 135 / 55.7 / 49.7;
+# 32 behind 16,000, 32/32 (32 rows): 1,016 / 111 / 86.
 PREFIX_LEAST_BYTES = 100 << 20
-PREFIX_STREAM_ROWS = 16
+PREFIX_STREAM_ROWS = 24
 
 
 def prefix_own_splits(seqs: int, n_heads: int, n_kv_heads: int, most_own: int, sms: int) -> int:
@@ -656,27 +661,37 @@ def prefix_own_splits(seqs: int, n_heads: int, n_kv_heads: int, most_own: int, s
 PREFIX_TC, PREFIX_STREAM, PREFIX_ROWS = 0, 1, 2
 
 
+def prefix_tc_pieces(seqs: int, group: int, n_kv_heads: int, sms: int) -> int:
+    """The most pieces of a prefix that the tcgen05 kernel cuts it into for single tokens of up to so many sequences."""
+    return min(32, max(4, sms // (-(-seqs // (2 * (128 // group))) * n_kv_heads)))
+
+
 def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, page_size: int) -> tuple[int, int, int]:
     """(pieces of a prefix, pieces of a sequence's own keys, kernel of the prefixes); of single tokens from the most sequences the
-    engine can hold (see `ops.prefix_plan`).  (n, 0, ..): prefix and own keys are one list in n pieces; (0, n, ..): every
+    engine can hold (see `ops.prefix_plan`), the families in the step and what the largest of them was, not from who is left of
+    them.  (n, 0, ..): prefix and own keys are one list in n pieces; (0, n, ..): every
     sequence reads its prefix by itself."""
     one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
     streams = one and page_size % 32 == 0 and group <= 16 and ctx.n_tokens == ctx.n_seqs
     if streams and seqs * g.most_len * n_kv_heads * head_dim * 4 <= PREFIX_LEAST_BYTES:
         return 0, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_len + g.most_own, sms), PREFIX_STREAM
-    rows = group * (getattr(ctx, "most_seqs", None) or g.most_tokens)
+    rows, shared = group * (getattr(g, "most_members", None) or g.most_tokens), getattr(g, "n_shared", None) or g.n_groups
     if streams and (rows <= PREFIX_STREAM_ROWS or page_size % 64):
         tiles = -(-seqs // (16 // group)) * n_kv_heads
         pieces = max(1, min(2 * sms // tiles, 32, -(-g.most_len // 256)))
         return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_STREAM
     if page_size % 64 == 0:                       # 256 query rows a block, one block an SM
         tile_tokens = 2 * (128 // group)
-        tiles = -(-seqs // tile_tokens) if one else ctx.n_tokens // tile_tokens + g.n_groups
-        most = sms // (tiles * n_kv_heads)
+        tiles = max(shared, -(-seqs // tile_tokens)) if one else ctx.n_tokens // tile_tokens + g.n_groups
         if not one:
-            return max(1, min(most, 32, (g.most_len + g.most_own) // 256)), 0, PREFIX_TC
-        return max(1, min(most, 32, -(-g.most_len // 128))), prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_TC
+            return max(1, min(sms // (tiles * n_kv_heads), 32, (g.most_len + g.most_own) // 256)), 0, PREFIX_TC
+        # as many pieces as end first: rounds of one block an SM, each its key blocks and about five key blocks' time besides
+        # (by the blocks of one full round 3 families of 16 behind 6,000 tokens, 32/8 heads, take 50.7 instead of 35.1 us)
+        blocks = -(-g.most_len // 128)
+        most = max(1, min(prefix_tc_pieces(seqs, group, n_kv_heads, sms), blocks))
+        pieces = min(range(1, most + 1), key=lambda n: -(-tiles * n_kv_heads * n // sms) * (-(-blocks // n) + 5))
+        return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_TC
     pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
     return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms) if streams else own, PREFIX_ROWS
 

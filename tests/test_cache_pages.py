@@ -137,6 +137,29 @@ def test_the_last_fork_counts():
     assert c.shared_prefixes([]) == [] and not c.shares
 
 
+def test_families_are_remembered_while_someone_is_left():
+    c = make()
+    a = c.acquire()
+    grow(c, a, 70)
+    b, d = c.fork(a, 2)
+    assert c.most_members([a, b, d]) == 3 and c.most_members([]) == 0
+    c.release(b)
+    c.release(d)
+    assert c.most_members([a]) == 3                   # who has ended counts on
+    for _ in range(5):                                # one after the other, never more than three at a time
+        (e,) = c.fork(a)
+        c.release(e)
+    assert c.most_members([a]) == 3 and len(c.families) == 1
+    grow(c, a, 30)
+    (e,) = c.fork(a)                                  # another fork: nobody is left of the first
+    assert c.most_members([a, e]) == 2 and len(c.families) == 1
+    c.truncate(e, 64)
+    assert c.most_members([e]) == 0 and c.most_members([a]) == 2
+    c.release(a)
+    c.release(e)
+    assert not c.families and not c.shares
+
+
 def test_random_traffic_with_forks_loses_nothing():
     rng = random.Random(5)
     c = make([KVNeed(2, 16), KVNeed(1, 32, window=100)], tokens=64 * 30, slots=9, ctx=700)

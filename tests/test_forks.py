@@ -97,6 +97,37 @@ def test_no_completion_is_refused():
         Generator(FakeEngine(2, 9), FakeSampler()).generate([[1]], 2, n=0)
 
 
+# ---- plans, on the CPU --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 128), (32, 32, 128), (64, 8, 64), (16, 1, 64), (100, 100, 128), (40, 2, 80)])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("slots", [1, 4, 24, 64, 300])
+def test_planned_scratch_takes_every_plan(heads, kv_heads, dim, page, slots):
+    """Whatever lengths and families a step of single tokens has, its parts fit what the engine planned; and they do not follow
+    from who is left of a family."""
+    from types import SimpleNamespace
+
+    from mdma_b200 import ops, ops_tensor
+    from mdma_b200.engine.step import prefix_floats
+    context = 20000
+    part = SimpleNamespace(prefix_shapes=lambda: [(heads, kv_heads, dim)])
+    have = prefix_floats(SimpleNamespace(all_parts=lambda: [part]), torch.bfloat16, 148, slots, context, page)
+    for length in (1024, 2048, 4096, 10240, context):
+        for families in (1, 2, 3, 7, 16, 100):
+            for members in (1, 2, 5, 16, 100):
+                if families * members > slots:
+                    continue
+                g = SimpleNamespace(most_len=length, most_own=context, most_tokens=members, n_groups=families, n_shared=families,
+                                    most_members=members)
+                live = slots - slots // 2
+                ctx = SimpleNamespace(max_new=1, n_seqs=slots, n_tokens=slots, most_seqs=slots)
+                fewer = SimpleNamespace(max_new=1, n_seqs=live, n_tokens=live, most_seqs=slots)
+                plan = ops_tensor.prefix_plan(ctx, g, heads, kv_heads, dim, 148, page)
+                assert 0 <= plan[0] <= 32 and 0 <= plan[1] <= 32
+                assert ops.prefix_scratch_floats(slots, heads, plan[0] + plan[1], dim) <= have
+                g.most_tokens = 1
+                assert ops_tensor.prefix_plan(fewer, g, heads, kv_heads, dim, 148, page) == plan
+
+
 # ---- the engine -----------------------------------------------------------------------------------------------------------------
 def step(eng, entries):
     from mdma_b200.engine import StepEntry
@@ -212,6 +243,89 @@ def test_replayed_steps_equal_steps_on_their_own(dtype):
     assert chosen == steps[False][1][:len(chosen)] and len(replayed) == len(runs)
     for n, logits in replayed.items():
         assert torch.equal(logits, steps[False][0][n])
+
+
+def shared_whatever_the_size(monkeypatch, rows):
+    """Prefixes of any size are shared in bfloat16, those of up to `rows` query rows streamed; returns the plans that are made."""
+    from mdma_b200 import ops_tensor
+    plans, plan_of = [], ops_tensor.prefix_plan
+    monkeypatch.setattr(ops_tensor, "PREFIX_LEAST_BYTES", 0)
+    monkeypatch.setattr(ops_tensor, "PREFIX_STREAM_ROWS", rows)
+
+    def noted(ctx, *args):
+        plans.append((ctx.max_new, plan_of(ctx, *args)))
+        return plans[-1][1]
+    monkeypatch.setattr(ops_tensor, "prefix_plan", noted)
+    return plans
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [0, 1 << 20], ids=["tcgen05", "streamed"])
+@pytest.mark.parametrize("cfg", [TINY_A, TINY_B, TINY_C, TINY_D, TINY_E], ids="ABCDE")
+def test_small_prefixes_through_the_kernels_of_large_ones(monkeypatch, cfg, rows):
+    plans = shared_whatever_the_size(monkeypatch, rows)
+    test_forked_sequences_against_the_plain_implementation("bfloat16", cfg, 64)
+    from mdma_b200 import ops_tensor
+    if ops_tensor.attention_supported(cfg["num_attention_heads"], cfg["num_key_value_heads"], cfg["head_dim"]):
+        group = cfg["num_attention_heads"] // cfg["num_key_value_heads"]
+        want = ops_tensor.PREFIX_STREAM if rows and group <= 16 else ops_tensor.PREFIX_TC
+        assert any(new == 1 and plan[0] > 0 and plan[2] == want for new, plan in plans)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [0, 1 << 20], ids=["tcgen05", "streamed"])
+def test_replayed_steps_through_the_kernels_of_large_prefixes(monkeypatch, rows):
+    plans = shared_whatever_the_size(monkeypatch, rows)
+    test_replayed_steps_equal_steps_on_their_own("bfloat16")
+    assert any(plan[0] > 0 for _, plan in plans)
+
+
+@pytest.mark.gpu
+def test_graphs_of_families_are_kept_within_bounds():
+    """Families of every size in turn, twice: the tokens are those of steps without graphs."""
+    from mdma_b200.engine import Engine
+    d, c, _ = make_model(TINY_D, 2, torch.bfloat16, std_scale=SHARP)
+    eng = Engine(d, dtype="float32", max_batch=6, max_context=256)
+    session = eng.decode_session()
+    session.most_prefix_graphs = 2
+    tokens = {}
+    for use_graph in (True, True, False):
+        for n in (1, 2, 3, 4, 5):
+            a = eng.acquire()
+            step(eng, [(a, ids(TINY_D, 70, n))])
+            slots = [a] + eng.fork(a, n)
+            session.start(slots, [3] * (n + 1))
+            got = []
+            while len(got) < 4:
+                session.run(1, use_graph=use_graph)
+                got += [t for t, _ in session.read()]
+            for s in slots:
+                eng.release(s)
+            assert tokens.setdefault(n, got) == got
+            assert sum(1 for key in session.graphs if len(key) > 3) <= 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [0, 1 << 20], ids=["tcgen05", "streamed"])
+def test_sums_stay_when_members_end(monkeypatch, rows):
+    """Bit for bit: a member's next logits, whether its mates are still there or have ended (six sequences of two kv heads, so that
+    the same warps take part)."""
+    from mdma_b200.engine import Engine
+    shared_whatever_the_size(monkeypatch, rows)
+    d, c, _ = make_model(TINY_D, 2, torch.bfloat16, std_scale=SHARP)
+    out = []
+    for stay in (6, 2):
+        eng = Engine(d, dtype="bfloat16", max_batch=6, max_context=2304)
+        a = eng.acquire()
+        step(eng, [(a, ids(TINY_D, 1021, 0))])
+        slots = [a] + eng.fork(a, 5)
+        got = [step(eng, [(s, [3 + i], [0]) for i, s in enumerate(slots)])]
+        for s in slots[stay:]:
+            eng.release(s)
+        for turn in range(3):
+            got.append(step(eng, [(s, [9 + turn], [0]) for s in slots[:stay]])[:2])
+        out.append(got)
+    assert all(np.array_equal(x[:2], y[:2]) for x, y in zip(*out))
 
 
 @pytest.mark.gpu
