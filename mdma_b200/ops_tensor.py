@@ -4,6 +4,7 @@ a shape the kernels refuse raises `KernelError`."""
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -666,6 +667,14 @@ def prefix_tc_pieces(seqs: int, group: int, n_kv_heads: int, sms: int) -> int:
     return min(32, max(4, sms // (-(-seqs // (2 * (128 // group))) * n_kv_heads)))
 
 
+@functools.lru_cache(maxsize=4096)
+def _tc_pieces(tiles: int, blocks: int, most: int, sms: int) -> int:
+    """Into how many pieces so many tiles' lists of key blocks are cut: as many as end first by rounds of one block an SM, each its key
+    blocks and about five key blocks' time besides.  (Cut for one full round of the engine's capacity, 3 families of 16 behind 6,000
+    tokens, 32/8 heads, take 50.7 instead of 35.1 us.)"""
+    return min(range(1, max(1, min(most, blocks)) + 1), key=lambda n: -(-tiles * n // sms) * (-(-blocks // n) + 5))
+
+
 def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, page_size: int) -> tuple[int, int, int]:
     """(pieces of a prefix, pieces of a sequence's own keys, kernel of the prefixes); of single tokens from the most sequences the
     engine can hold (see `ops.prefix_plan`), the families in the step and what the largest of them was, not from who is left of
@@ -686,11 +695,7 @@ def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, 
         tiles = max(shared, -(-seqs // tile_tokens)) if one else ctx.n_tokens // tile_tokens + g.n_groups
         if not one:
             return max(1, min(sms // (tiles * n_kv_heads), 32, (g.most_len + g.most_own) // 256)), 0, PREFIX_TC
-        # as many pieces as end first: rounds of one block an SM, each its key blocks and about five key blocks' time besides
-        # (by the blocks of one full round 3 families of 16 behind 6,000 tokens, 32/8 heads, take 50.7 instead of 35.1 us)
-        blocks = -(-g.most_len // 128)
-        most = max(1, min(prefix_tc_pieces(seqs, group, n_kv_heads, sms), blocks))
-        pieces = min(range(1, most + 1), key=lambda n: -(-tiles * n_kv_heads * n // sms) * (-(-blocks // n) + 5))
+        pieces = _tc_pieces(tiles * n_kv_heads, -(-g.most_len // 128), prefix_tc_pieces(seqs, group, n_kv_heads, sms), sms)
         return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_TC
     pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
     return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms) if streams else own, PREFIX_ROWS
