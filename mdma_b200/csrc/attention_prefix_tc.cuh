@@ -18,7 +18,7 @@
 // row (the issue slots of sixteen softmax warps are the bound then) 4,200; a warp that issues for each tile, both in step, 4,850;
 // P V behind the whole softmax 3,450; steps of 64 keys with two places for S (products of N = 64 cost as much as of N = 128)
 // 3,700; the first half's weights before the row's maximum is known 3,450; a quarter of the exponentials by a polynomial on the
-// multiply-add units 3,400; the next blocks asked into L2 ahead, 15% more where they come from memory.
+// multiply-add units 3,400; the two tiles' exponentials in turns (a barrier for every pair of warps) 3,650; the next blocks asked into L2 ahead, 15% more where they come from memory.
 // 8,960 rows a kv head over 8,000 keys, 32 heads of 128: 320 us, 1.0 PFLOP/s.
 //
 // The list: the prefix's blocks, which all rows see, and (`whole`) behind them the own blocks of every sequence with tokens in the
