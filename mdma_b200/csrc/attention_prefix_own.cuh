@@ -217,8 +217,8 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         float l = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const float f = mine[u].x == -INFINITY ? -1.f : exp2f(mine[u].x - m);     // who has no keys has no share
-            if (f >= 0.f) l += f * mine[u].y;
+            const float f = prefix_share(mine[u], m);
+            if (prefix_joins(f)) l += f * mine[u].y;
             if (u * 32 + lane < NW + used) share[(u * 32 + lane) * 16 + r] = f;
         }
         l = warp_sum(l);
@@ -233,7 +233,7 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const float l = row_l[r];
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         auto join = [&](float f, const float4& x) {
-            if (f >= 0.f) { acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w); }
+            if (prefix_joins(f)) { acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w); }
         };
         const size_t row = row_of(r);
         const float* part = p.part_o + row * slots * D + d;

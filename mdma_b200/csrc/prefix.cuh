@@ -79,6 +79,11 @@ static inline long prefix_tiles_bound(const PrefixParams& p, int tile_tokens) {
     return (long)p.n_tokens / tile_tokens + p.n_groups;
 }
 
+// A part's share of the whole, 2^(its maximum - m).  -1, no share: a part without keys leaves no maximum and no sum.  (The
+// maximum passes over NaN: a part whose scores are all NaN leaves no maximum either, but a sum that is NaN, and joins.)
+__device__ __forceinline__ float prefix_share(float2 ml, float m) { return ml.x == -INFINITY && ml.y == 0.f ? -1.f : exp2f(ml.x - m); }
+__device__ __forceinline__ bool prefix_joins(float share) { return !(share < 0.f); }
+
 // out[token, head] from its parts: those of its prefix in order, then those of its own keys.  One warp for 64 numbers of a row: a lane
 // a part for the maxima, the sums and the shares (at most 64 parts), then all lanes over the parts' numbers, eight parts in flight.
 template <typename T>
@@ -100,8 +105,8 @@ prefix_merge_kernel(const PrefixParams p) {
     float share[2], l = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        share[u] = mine[u].x == -INFINITY ? -1.f : exp2f(mine[u].x - m);              // a part without keys has no share
-        if (share[u] >= 0.f) l += share[u] * mine[u].y;
+        share[u] = prefix_share(mine[u], m);
+        if (prefix_joins(share[u])) l += share[u] * mine[u].y;
     }
     l = warp_sum(l);
     if (p.sinks) l += exp2f(p.sinks[row % p.n_heads] * p.sink_rate - m);
@@ -122,7 +127,7 @@ prefix_merge_kernel(const PrefixParams p) {
             for (int u = 0; u < 8; ++u) {
                 const int s = s0 + u;
                 const float f = __shfl_sync(0xffffffffu, s < 32 ? share[0] : share[1], s & 31);
-                if (s < parts && f >= 0.f) { a0 = fmaf(f, x0[u], a0); a1 = fmaf(f, x1[u], a1); }
+                if (s < parts && prefix_joins(f)) { a0 = fmaf(f, x0[u], a0); a1 = fmaf(f, x1[u], a1); }
             }
         }
         if (one) to[d] = from_float<T>(a0 / l);
