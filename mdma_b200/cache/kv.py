@@ -243,6 +243,8 @@ class SequenceCache:
             return ValueError(f"a sequence of {old} tokens cannot fork at {length}")
         if length != old and self.state_bytes:
             return ValueError("a cache with fixed-size per-sequence state forks at a sequence's end only")
+        if any(not s.is_cuda for s in self.states.values()):
+            return ValueError("state is copied on the GPU only: this cache lies elsewhere")
         if n > self.slots.free_count:
             return CacheFull(f"{n} more sequence slots are wanted, {self.slots.free_count} of {self.slots.n} are free")
         for g in self.groups:
@@ -281,24 +283,31 @@ class SequenceCache:
         length = self.lengths[slot] if length is None else length
         new = [self.slots.acquire() for _ in range(n)]
         full, rows = divmod(length, self.page_size)
-        for g in self.groups:
-            have = g.seq_pages.get(slot, {})
-            first = g.need.first_key(length) // self.page_size if g.need.bounded else 0
-            for p, page in have.items():
-                if p < full and (p >= first or p < g.kept_pages):
-                    g.holders[page] = g.holders.get(page, 1) + n
-                    for s in new:
-                        g.place(s, p, page)
-            if rows and full in have:
-                copies = g.pages.acquire_many(n)
-                for s, page in zip(new, copies):
-                    g.place(s, full, page)
-                g.copy([have[full]] * n, copies, [rows] * n)
-            g.sync_tables()
-        if self.states:
-            from .. import ops
-            with torch.cuda.device(self.device):
-                ops.copy_slots(list(self.states.values()), [slot] * n, new)
+        try:
+            for g in self.groups:
+                have = g.seq_pages.get(slot, {})
+                first = g.need.first_key(length) // self.page_size if g.need.bounded else 0
+                for p, page in have.items():
+                    if p < full and (p >= first or p < g.kept_pages):
+                        g.holders[page] = g.holders.get(page, 1) + n
+                        for s in new:
+                            g.place(s, p, page)
+                if rows and full in have:
+                    copies = g.pages.acquire_many(n)
+                    for s, page in zip(new, copies):
+                        g.place(s, full, page)
+                    g.copy([have[full]] * n, copies, [rows] * n)
+                g.sync_tables()
+            if self.states:
+                from .. import ops
+                with torch.cuda.device(self.device):
+                    ops.copy_slots(list(self.states.values()), [slot] * n, new)
+        except BaseException:
+            for s in new:                                   # a copy failed: what was taken goes back
+                self.slots.release(s)
+                for g in self.groups:
+                    g.release(s)
+            raise
         for s in new:
             self.lengths[s] = length
         if length:
