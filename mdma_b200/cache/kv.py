@@ -435,16 +435,30 @@ class SequenceCache:
                 raise ValueError("pages are copied on the GPU only: this cache lies elsewhere")
             if g.pages.free_count + sum(1 for p, page in g.seq_pages[slot].items() if p > last and page not in g.holders) < 1:
                 raise CacheFull(f"a page for the kept rows of a shared one is wanted, none of {g.n_pages} is free")
+        # the copies come before any page is given back, so that one that fails leaves the sequence as it was: a copy goes to a
+        # page of the sequence's own beyond the kept rows (its number is noted), or else to a free one
+        copies = []
+        for g in own:
+            beyond = next((p for p, page in g.seq_pages[slot].items() if p > last and page not in g.holders), None)
+            copies.append((g, g.pages.acquire() if beyond is None else g.seq_pages[slot][beyond], beyond))
+        try:
+            for g, page, _ in copies:
+                g.copy([g.seq_pages[slot][last]], [page], [rows])
+        except BaseException:
+            for g, page, beyond in copies:
+                if beyond is None:
+                    g.pages.release(page)
+            raise
+        for g, page, beyond in copies:
+            if beyond is not None:
+                del g.seq_pages[slot][beyond]
+            g.drop(g.seq_pages[slot][last])
+            g.place(slot, last, page)
+            g.sync_tables()
         for g in self.groups:
             have = g.seq_pages.get(slot, {})
             for p in [p for p in have if p > last]:
                 g.drop(have.pop(p))
-            if g in own:
-                (page,) = g.pages.acquire_many(1)
-                g.copy([have[last]], [page], [rows])
-                g.drop(have[last])
-                g.place(slot, last, page)
-                g.sync_tables()
         if self.shares.get(slot, (0, 0))[1] > length:
             self._share(slot, None)                 # it has less than its fork shares
         self.lengths[slot] = length

@@ -62,3 +62,32 @@ def test_a_fork_whose_copies_fail_gives_everything_back(fails, monkeypatch):
     c.release(b)
     c.check()
     assert all(g.pages.free_count == g.n_pages for g in c.groups)
+
+
+@pytest.mark.parametrize("free", [0, 3])
+def test_a_truncation_whose_copy_fails_changes_nothing(free, monkeypatch):
+    c = make([KVNeed(2, 16), KVNeed(1, 8)], [None, None], allocate=False, tokens=64 * (5 + free))
+    a = c.acquire()
+    grow(c, a, 192)
+    (b,) = c.fork(a)
+    grow(c, b, 100)                                  # two pages of its own behind the shared ones
+    calls = []
+
+    def copy(*args):
+        calls.append(args)
+        if len(calls) == 2:
+            raise RuntimeError("no copy")
+    monkeypatch.setattr(CacheGroup, "copy", copy)
+    before = books(c)
+    with pytest.raises(RuntimeError, match="no copy"):
+        c.truncate(b, 100)
+    c.check()
+    assert books(c) == before
+    calls.clear()
+    calls.append(None)
+    monkeypatch.setattr(CacheGroup, "copy", lambda *args: calls.append(args))
+    c.truncate(b, 100)
+    c.check()
+    for (group, src, dst, rows), g in zip(calls[1:], c.groups):
+        assert group is g and src == [g.seq_pages[a][1]] and dst == [g.seq_pages[b][1]] and rows == [36] and src != dst
+    assert len(calls) == 3 and c.length(b) == 100 and all(sorted(g.seq_pages[b]) == [0, 1] for g in c.groups)
