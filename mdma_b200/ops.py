@@ -1228,11 +1228,14 @@ def prefix_checks(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: in
         raise KernelError("queries, caches, results and sinks are on one device")
     for t in (ctx.seq_start, ctx.seq_pos0, ctx.seq_slot, ctx.tok_seq, view.page_table, g.group_len, g.group_seq, g.tok_first, g.toks,
               g.seq_skip):
-        if t.dtype is not int32 or t.get_device() != device:
-            raise KernelError("positions, page tables and groups are int32, on the queries' device")
+        if t.dtype is not int32 or t.get_device() != device or not t.is_contiguous():
+            raise KernelError("positions, page tables and groups are contiguous int32, on the queries' device")
+    table = view.page_table.shape
+    if len(table) != 2 or table[1] != view.max_pages:
+        raise KernelError(f"a page table of {tuple(table)} does not hold {view.max_pages} pages a slot")
     dtype, rows, shape = q.dtype, q.shape, out.shape
     if (k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or len(rows) != 2 or q.stride(1) != 1
-            or not (k.is_contiguous() and v.is_contiguous() and out.is_contiguous() and view.page_table.is_contiguous())):
+            or not (k.is_contiguous() and v.is_contiguous() and out.is_contiguous())):
         raise KernelError("queries, caches and results have one dtype; caches and results are contiguous")
     if (n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads or len(k.shape) != 4 or k.shape != v.shape
             or k.size(1) != view.page_size or k.size(2) != n_kv_heads or k.size(3) != head_dim or len(shape) != 2
