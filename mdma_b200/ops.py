@@ -1182,10 +1182,18 @@ def _prefix_rows(rows: int) -> int:
     return 8 if rows <= 8 else 32 if rows <= 32 else 64
 
 
+def prefix_tile_rows(ctx, g, group: int) -> tuple[int, int]:
+    """(query rows a block of the prefixes takes, of the own keys) on the CUDA cores.  Of single tokens they follow from the most
+    members that the largest family of the step has had, not from who is left of it: another tile adds up in another order."""
+    tokens = (getattr(g, "most_members", None) or g.most_tokens) if ctx.max_new == 1 else ctx.n_tokens
+    return _prefix_rows(tokens * group), _prefix_rows(ctx.max_new * group)
+
+
 def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, sms: int = 148) -> tuple[int, int]:
     """(pieces of a prefix, pieces of a sequence's own keys) of a step on the CUDA cores, 32 keys each at least, for about four
-    blocks an SM (two of 64 rows, which is what its shared memory takes).  Of single tokens it follows from the most sequences the engine can hold, not from the live ones, so that a
-    request's sums are cut at the same places when a batch mate ends."""
+    blocks an SM (two of 64 rows, which is what its shared memory takes).  Of single tokens it follows from the most sequences the
+    engine can hold, not from the live ones, so that a request's sums are cut at the same places when a batch mate ends (which
+    tile works them off: `prefix_tile_rows`)."""
     one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
     tokens = seqs if one else ctx.n_tokens
@@ -1269,6 +1277,6 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.get_device() != q.get_device():
         raise KernelError(f"prefix attention needs {need} floats of scratch on the queries' device, {scratch.numel()} given")
     words = prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sinks, None, False)
-    group = n_heads // n_kv_heads
+    rows, own_rows = prefix_tile_rows(ctx, g, n_heads // n_kv_heads)
     _call("core", "mdma_prefix_attention_simple", ctypes.c_void_p(words.buffer_info()[0]), _i(32), _f(scale), _i(dtype_code(q.dtype)),
-          _i(_prefix_rows(ctx.n_tokens * group)), _i(_prefix_rows(ctx.max_new * group)), _stream(), launches=3)
+          _i(rows), _i(own_rows), _stream(), launches=3)
