@@ -23,7 +23,7 @@ struct PoSmem {
     static constexpr int kTile = KB * DMAX * 2, kRow = DMAX + 8;                      // bytes of a tile; floats of a warp's row of sums
     static constexpr int kTiles = NW * 2 * kTile, kComb = NW * 16 * kRow * 4;
     static constexpr int kQ = kTiles > kComb ? kTiles : kComb, kBars = kQ + 16 * DMAX * 2, kTop = kBars + NW * 16 + 16;
-    static constexpr int kBytes = kTop + (3 * NW + kPoMaxPieces + 2) * 16 * 4;
+    static constexpr int kBytes = kTop + (3 * NW + kPoMaxPieces + 3) * 16 * 4;
 };
 
 template <int DMAX, int KB, int NW, bool SHARED>
@@ -63,8 +63,7 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const int end = p.seq_pos0[seq] + 1;
         token = seq;                                             // (every sequence brings one)
         skip = p.pieces > 0 ? p.seq_skip[seq] : 0;
-        const int per = ((end - skip + p.own_splits - 1) / p.own_splits + KB - 1) / KB * KB;
-        lo = skip + split * per; hi = min(end, lo + per);
+        own_piece(p, skip, end, split, KB, lo, hi);
     }
     const int* pages = p.page_table + (size_t)p.seq_slot[seq] * p.max_pages;
     // the token of a row of the tile
@@ -179,12 +178,13 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 1); l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 2);
     l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 1); l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 2);
 
-    // ---- join: warps in their order, then the prefix's parts in theirs -----------------------------------------------
+    // ---- join: the warps in their order, then the prefix's parts in theirs and what the warps made behind them (as the merge
+    // kernel joins them, so that it does not matter to a sequence which of the two does) -------------------------------
     __syncthreads();                                             // the tiles are read: their place takes the warps' sums
     float* comb = reinterpret_cast<float*>(smem);
     float* top = reinterpret_cast<float*>(smem + L::kTop);       // [NW][16] maxima, [NW][16] sums of the warps
-    float* share = top + 2 * NW * 16;                            // [NW + pieces][16] shares of the warps and of the prefix's parts
-    float *row_m = share + (NW + kPoMaxPieces) * 16, *row_l = row_m + 16;
+    float* share = top + 2 * NW * 16;                            // [NW + pieces + 1][16] shares of the warps, of the prefix's parts and of the own keys
+    float *row_m = share + (NW + kPoMaxPieces + 1) * 16, *row_l = row_m + 16;
     {
         float* mine = comb + (size_t)warp * 16 * L::kRow;
         const int r_lo = lane >> 2, r_hi = r_lo + 8;
@@ -204,35 +204,40 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     auto row_of = [&](int r) { return (size_t)token_of(r) * p.n_heads + kvh * G + r % G; };
     if (!SHARED) chain_wait();                                   // the prefixes' parts are there, and all that was waited for before them
     __syncthreads();
-    // a warp a row: the maximum of the warps' and the parts' maxima, everyone's share, the sum (a lane a contribution, up to two)
+    // a warp a row: the warps' maxima, shares and sum (a lane a warp), then those of the prefix's parts and the own keys (a lane a
+    // contribution, up to two)
     for (int r = warp; r < rows; r += NW) {
         const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row_of(r) * slots;
-        float2 mine[2];
+        float2 part[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int i = u * 32 + lane;
-            mine[u] = i < NW ? make_float2(top[i * 16 + r], top[(NW + i) * 16 + r]) : i < NW + used ? __ldcg(ml + i - NW) : make_float2(-INFINITY, 0.f);
-        }
-        const float m = warp_max(fmaxf(mine[0].x, mine[1].x));
-        float l = 0.f;
+        for (int u = 0; u < 2; ++u) part[u] = u * 32 + lane < used ? __ldcg(ml + u * 32 + lane) : make_float2(-INFINITY, 0.f);
+        const float2 mine = lane < NW ? make_float2(top[lane * 16 + r], top[(NW + lane) * 16 + r]) : make_float2(-INFINITY, 0.f);
+        float m = warp_max(mine.x);
+        const float f = prefix_share(mine, m);
+        float l = warp_sum(prefix_joins(f) ? f * mine.y : 0.f);
+        if (lane < NW) share[lane * 16 + r] = f;
+        if (joins) {
+            const float2 own = make_float2(m, l);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float f = prefix_share(mine[u], m);
-            if (prefix_joins(f)) l += f * mine[u].y;
-            if (u * 32 + lane < NW + used) share[(u * 32 + lane) * 16 + r] = f;
+            for (int u = 0; u < 2; ++u) if (u * 32 + lane == used) part[u] = own;
+            m = warp_max(fmaxf(part[0].x, part[1].x));
+            l = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float g = prefix_share(part[u], m);
+                if (prefix_joins(g)) l += g * part[u].y;
+                if (u * 32 + lane <= used) share[(NW + u * 32 + lane) * 16 + r] = g;
+            }
+            l = warp_sum(l);
+            if (p.sinks) l += exp2f(p.sinks[kvh * G + r % G] * p.sink_rate - m);
         }
-        l = warp_sum(l);
-        if (lane == 0) {
-            if (joins && p.sinks) l += exp2f(p.sinks[kvh * G + r % G] * p.sink_rate - m);
-            row_m[r] = m; row_l[r] = l;
-        }
+        if (lane == 0) { row_m[r] = m; row_l[r] = l; }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 32) {
         const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
         const float l = row_l[r];
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto join = [&](float f, const float4& x) {
+        auto join = [&](float f, const float4& x, float4& acc) {
             if (prefix_joins(f)) { acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w); }
         };
         const size_t row = row_of(r);
@@ -243,19 +248,22 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             for (int u = 0; u < 8; ++u) x[u] = __ldcg(reinterpret_cast<const float4*>(part + (size_t)min(s0 + u, used - 1) * D));
         };
         if (used > 0) fetch(0);
+        float4 own = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) join(share[w * 16 + r], *reinterpret_cast<const float4*>(comb + ((size_t)w * 16 + r) * L::kRow + d));
-        for (int s0 = 0; s0 < used; s0 += 8) {
-            if (s0 > 0) fetch(s0);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) if (s0 + u < used) join(share[(NW + s0 + u) * 16 + r], x[u]);
-        }
+        for (int w = 0; w < NW; ++w) join(share[w * 16 + r], *reinterpret_cast<const float4*>(comb + ((size_t)w * 16 + r) * L::kRow + d), own);
         if (joins) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s0 = 0; s0 < used; s0 += 8) {
+                if (s0 > 0) fetch(s0);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) if (s0 + u < used) join(share[(NW + s0 + u) * 16 + r], x[u], acc);
+            }
+            join(share[(NW + used) * 16 + r], own, acc);
             __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x / l, acc.y / l), __floats2bfloat162_rn(acc.z / l, acc.w / l)};
             *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * D + d) = *reinterpret_cast<const uint2*>(y);
         } else {
             const size_t slot = row * slots + (SHARED ? 0 : p.pieces) + split;
-            *reinterpret_cast<float4*>(p.part_o + slot * D + d) = acc;
+            *reinterpret_cast<float4*>(p.part_o + slot * D + d) = own;
             if (d == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(row_m[r], l);
         }
     }

@@ -23,6 +23,7 @@ struct PrefixParams {
     int n_groups, n_seqs, n_tokens, max_new;
     int n_heads, n_kv_heads, head_dim, group;
     int pieces, own_splits;                          // a prefix in `pieces` pieces at most, own keys in `own_splits`: slots of the parts
+    int own_keys;                                    // of single tokens: keys of a piece of the own keys, the last takes the rest (0: equal pieces)
     int unit;                                        // a piece of a prefix is a multiple of so many keys
     int whole;                                       // own_splits 0: all keys of a row tile, prefix and own ones, are one list in `pieces` pieces
     float scale_log2;                                // scale * log2(e)
@@ -39,6 +40,15 @@ __host__ __device__ __forceinline__ int prefix_pieces_used(int len, int pieces, 
     if (len <= 0) return 0;
     const int keys = prefix_piece(len, pieces, unit);
     return (len + keys - 1) / keys;
+}
+
+// Piece `split` of a sequence's own keys [skip, end): keys [lo, hi), of a multiple of `unit`.  Pieces of a fixed length are the same
+// whoever shares the step (only how many a step has room for follows from its longest sequence); most are empty beside one
+// long sequence.
+__device__ __forceinline__ void own_piece(const PrefixParams& p, int skip, int end, int split, int unit, int& lo, int& hi) {
+    const int keys = p.own_keys > 0 ? p.own_keys : ((end - skip + p.own_splits - 1) / p.own_splits + unit - 1) / unit * unit;
+    lo = skip + split * keys;
+    hi = p.own_keys > 0 && split == p.own_splits - 1 ? end : min(end, lo + keys);
 }
 
 // Tile t of the prefixes' query rows, `tile_tokens` tokens each: which group, which of its tokens.  Groups without a prefix
@@ -142,7 +152,7 @@ static inline unsigned prefix_merge_blocks(const PrefixParams& p) {
 // The arguments as one array of 64-bit words, in the order below (a step makes this call once a layer: converting thirty
 // arguments one by one costs the host more than the launches).
 static inline int prefix_params(const long long* w, int n_words, float scale, PrefixParams* out) {
-    MDMA_REQUIRE(n_words == 32, "prefix_attention: %d argument words", n_words);
+    MDMA_REQUIRE(n_words == 33, "prefix_attention: %d argument words", n_words);
     PrefixParams& p = *out;
     int i = 0;
     auto ptr = [&]() { return (void*)(uintptr_t)w[i++]; };
@@ -158,7 +168,7 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     const long long floats = w[i++];
     p.n_groups = num(); p.n_seqs = num(); p.n_tokens = num(); p.max_new = num();
     p.n_heads = num(); p.n_kv_heads = num(); p.head_dim = num();
-    p.pieces = num(); p.own_splits = num();
+    p.pieces = num(); p.own_splits = num(); p.own_keys = num();
     p.sinks = (const float*)ptr();
     p.status = (int*)ptr();
     p.sink_rate = w[i++] ? 1.0f : 1.4426950408889634f;      // the sinks come times log2(e), or as they are
@@ -166,7 +176,7 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     MDMA_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0, "prefix_attention: %d heads over %d kv heads", p.n_heads, p.n_kv_heads);
     MDMA_REQUIRE(p.head_dim > 0 && p.head_dim <= 256, "prefix_attention: head_dim %d is beyond the limit of 256", p.head_dim);
     MDMA_REQUIRE(p.page_table && p.page_size > 0 && p.max_pages > 0, "prefix_attention: bad cache geometry");
-    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 0 && p.own_splits >= 0 && p.pieces + p.own_splits > 0, "prefix_attention: bad sizes");
+    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 0 && p.own_splits >= 0 && p.own_keys >= 0 && p.pieces + p.own_splits > 0, "prefix_attention: bad sizes");
     MDMA_REQUIRE(p.pieces <= 32 && p.own_splits <= 32, "prefix_attention: %d and %d pieces are beyond the limit of 32", p.pieces, p.own_splits);
     MDMA_REQUIRE(scale > 0.f, "prefix_attention: the score scale must be positive");
     p.group = p.n_heads / p.n_kv_heads;

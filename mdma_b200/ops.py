@@ -1212,7 +1212,7 @@ def prefix_scratch_floats(tokens: int, n_heads: int, parts: int, head_dim: int) 
 
 
 def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, pieces: int, own_splits: int, scratch, sinks, status,
-                 sinks_log2: bool):
+                 sinks_log2: bool, own_keys: int = 0):
     """The arguments of the prefix attention kernels as one array (see csrc/prefix.cuh)."""
     g = ctx.prefix
     return array.array("q", (
@@ -1220,7 +1220,7 @@ def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int
         ctx.seq_slot.data_ptr(), ctx.tok_seq.data_ptr(), view.page_table.data_ptr(), view.max_pages, view.page_size,
         view.k.size(0), g.group_len.data_ptr(), g.group_seq.data_ptr(), g.tok_first.data_ptr(), g.toks.data_ptr(),
         g.seq_skip.data_ptr(), out.data_ptr(), scratch.data_ptr(), scratch.numel(), g.n_groups, ctx.n_seqs, ctx.n_tokens,
-        ctx.max_new, n_heads, n_kv_heads, head_dim, pieces, own_splits, 0 if sinks is None else sinks.data_ptr(),
+        ctx.max_new, n_heads, n_kv_heads, head_dim, pieces, own_splits, own_keys, 0 if sinks is None else sinks.data_ptr(),
         0 if status is None else status.data_ptr(), int(sinks_log2)))
 
 
@@ -1278,5 +1278,5 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
         raise KernelError(f"prefix attention needs {need} floats of scratch on the queries' device, {scratch.numel()} given")
     words = prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sinks, None, False)
     rows, own_rows = prefix_tile_rows(ctx, g, n_heads // n_kv_heads)
-    _call("core", "mdma_prefix_attention_simple", ctypes.c_void_p(words.buffer_info()[0]), _i(32), _f(scale), _i(dtype_code(q.dtype)),
+    _call("core", "mdma_prefix_attention_simple", ctypes.c_void_p(words.buffer_info()[0]), _i(len(words)), _f(scale), _i(dtype_code(q.dtype)),
           _i(rows), _i(own_rows), _stream(), launches=3)

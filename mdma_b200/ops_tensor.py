@@ -648,14 +648,27 @@ PREFIX_LEAST_BYTES = 100 << 20
 PREFIX_STREAM_ROWS = 24
 
 
-def prefix_own_splits(seqs: int, n_heads: int, n_kv_heads: int, most_own: int, sms: int) -> int:
-    """Into how many pieces a single token's own keys are cut: one block a (sequence, kv head) joins everything itself unless
-    the blocks leave most of the device idle and have more than a thousand keys each."""
-    if n_heads // n_kv_heads > 16:
-        return ops.prefix_split(64, 2 * sms, seqs, seqs, 1, 0, most_own, n_heads, n_kv_heads)[1]
-    if seqs * n_kv_heads * 2 > sms or most_own <= 1024:
-        return 1
-    return max(1, min(sms // (seqs * n_kv_heads), most_own // 512, 16))
+# Keys of a piece of the own keys of single tokens, at least, and what sequences x pieces may come to.
+PREFIX_OWN_KEYS = 1024
+PREFIX_OWN_PARTS = 512
+
+
+def prefix_streams(ctx, group: int, page_size: int) -> bool:
+    """Whether the step is one of single tokens that the streaming kernel takes."""
+    return ctx.max_new == 1 and page_size % 32 == 0 and group <= 16 and ctx.n_tokens == ctx.n_seqs
+
+
+def prefix_own_cut(ctx, most_own: int) -> tuple[int, int]:
+    """(pieces, keys of a piece) of the own keys of single tokens that are streamed: one block a (sequence, kv head) joins
+    everything itself up to a piece's keys.  Keys beyond are cut into pieces of a fixed length, so that a step does not wait for the
+    one long sequence's blocks; the length, a multiple of 1,024, follows from the most sequences and the longest context that the
+    engine can hold.  Only their number follows from the live ones: a sequence's keys are cut at the same places, and its parts
+    joined in the same order, whoever shares the step."""
+    seqs = getattr(ctx, "most_seqs", None) or ctx.n_seqs
+    most = max(1, min(PREFIX_OWN_PARTS // seqs, 16))
+    longest = max(most_own, getattr(ctx, "most_len", None) or 0)
+    keys = -(-longest // (most * PREFIX_OWN_KEYS)) * PREFIX_OWN_KEYS
+    return max(1, min(most, -(-most_own // keys))), keys
 
 
 # who does the prefixes (csrc/attention_prefix.cu)
@@ -676,29 +689,30 @@ def _tc_pieces(tiles: int, blocks: int, most: int, sms: int) -> int:
 
 
 def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, page_size: int) -> tuple[int, int, int]:
-    """(pieces of a prefix, pieces of a sequence's own keys, kernel of the prefixes); of single tokens from the most sequences the
-    engine can hold (see `ops.prefix_plan`), the families in the step and what the largest of them was, not from who is left of
-    them.  (n, 0, ..): prefix and own keys are one list in n pieces; (0, n, ..): every
-    sequence reads its prefix by itself."""
+    """(pieces of a prefix, pieces of a sequence's own keys, kernel of the prefixes); of single tokens from the most sequences and
+    the longest context the engine can hold (see `ops.prefix_plan`), the families in the step and what the largest of them was, not from
+    who is left of them (for the number of pieces of streamed own keys see `prefix_own_cut`).  (n, 0, ..): prefix and own keys are
+    one list in n pieces; (0, n, ..): every sequence reads its prefix by itself."""
     one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
-    streams = one and page_size % 32 == 0 and group <= 16 and ctx.n_tokens == ctx.n_seqs
+    streams = prefix_streams(ctx, group, page_size)
     if streams and seqs * g.most_len * n_kv_heads * head_dim * 4 <= PREFIX_LEAST_BYTES:
-        return 0, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_len + g.most_own, sms), PREFIX_STREAM
+        return 0, prefix_own_cut(ctx, g.most_len + g.most_own)[0], PREFIX_STREAM
+    most_own = max(g.most_own, getattr(ctx, "most_len", None) or 0) if one else g.most_own
+    pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, most_own, n_heads, n_kv_heads)
+    if streams:
+        own = prefix_own_cut(ctx, g.most_own)[0]
     rows, shared = group * (getattr(g, "most_members", None) or g.most_tokens), getattr(g, "n_shared", None) or g.n_groups
     if streams and (rows <= PREFIX_STREAM_ROWS or page_size % 64):
         tiles = -(-seqs // (16 // group)) * n_kv_heads
-        pieces = max(1, min(2 * sms // tiles, 32, -(-g.most_len // 256)))
-        return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_STREAM
+        return max(1, min(2 * sms // tiles, 32, -(-g.most_len // 256))), own, PREFIX_STREAM
     if page_size % 64 == 0:                       # 256 query rows a block, one block an SM
         tile_tokens = 2 * (128 // group)
         tiles = max(shared, -(-seqs // tile_tokens)) if one else ctx.n_tokens // tile_tokens + g.n_groups
         if not one:
             return max(1, min(sms // (tiles * n_kv_heads), 32, (g.most_len + g.most_own) // 256)), 0, PREFIX_TC
-        pieces = _tc_pieces(tiles * n_kv_heads, -(-g.most_len // 128), prefix_tc_pieces(seqs, group, n_kv_heads, sms), sms)
-        return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms), PREFIX_TC
-    pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, g.most_own, n_heads, n_kv_heads)
-    return pieces, prefix_own_splits(seqs, n_heads, n_kv_heads, g.most_own, sms) if streams else own, PREFIX_ROWS
+        return _tc_pieces(tiles * n_kv_heads, -(-g.most_len // 128), prefix_tc_pieces(seqs, group, n_kv_heads, sms), sms), own, PREFIX_TC
+    return pieces, own, PREFIX_ROWS
 
 
 def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
@@ -717,12 +731,16 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     flush_pending(q.device, st)
     g = ctx.prefix
     pieces, own, kind = prefix_plan(ctx, g, n_heads, n_kv_heads, head_dim, st.sms, view.page_size)
+    own_keys = 0
+    if own > 0 and prefix_streams(ctx, n_heads // n_kv_heads, view.page_size):
+        own_keys = prefix_own_cut(ctx, g.most_own + (0 if pieces else g.most_len))[1]
     need = ops.prefix_scratch_floats(ctx.n_tokens, n_heads, pieces + own, head_dim) if pieces + own > 1 else 0
     if own_st is not None:
         st.need(need, "attention over shared prefixes")
         scratch = st.scratch
     else:
         scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else out        # (nothing is kept there)
-    words = ops.prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sink_log2, st.status, True)
-    _call("tensor", "mdma_prefix_attention", ctypes.c_void_p(words.buffer_info()[0]), _i(32), _f(scale), _i(kind), _stream(),
+    words = ops.prefix_words(ctx, q, view, out, n_heads, n_kv_heads, head_dim, pieces, own, scratch, sink_log2, st.status, True,
+                             own_keys)
+    _call("tensor", "mdma_prefix_attention", ctypes.c_void_p(words.buffer_info()[0]), _i(len(words)), _f(scale), _i(kind), _stream(),
           launches=(pieces > 0) + (own > 0) + (pieces > 1 if own == 0 else own > 1 or ctx.max_new > 1 or n_heads // n_kv_heads > 16 or view.page_size % 32 != 0))
