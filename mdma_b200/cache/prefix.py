@@ -49,7 +49,7 @@ class PrefixGroups:
         self.most_members = max((len(members) for length, members in groups if length), default=0)
         self.most_tokens = max(sizes, default=0)
         self.most_len = max((length for length, _ in groups), default=0)
-        self.least_skip = min(skip, default=0)
+        self.skips = skip
         self.most_own = max((p + t - s for p, t, s in zip(pos0, new, skip)), default=0)
         self._host = {"group_len": [length for length, _ in groups], "group_seq": [members[0] for _, members in groups],
                       "tok_first": np.concatenate([[0], np.cumsum(sizes)]) if groups else [0],

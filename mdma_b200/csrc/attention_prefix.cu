@@ -220,7 +220,8 @@ template <bool SHARED>
 static int launch_prefix_stream(const PrefixParams& p, int sms, cudaStream_t stream) {
     const int kb = p.head_dim <= 64 && p.page_size % 64 == 0 ? 64 : 32;       // a tile of 8 KB either way
     const long items = SHARED ? prefix_tiles_bound(p, 16 / p.group) : p.n_seqs, splits = SHARED ? p.pieces : p.own_splits;
-    const long blocks = p.n_kv_heads * splits * (SHARED ? (p.n_tokens * p.group + 15) / 16 : items);       // (those that have something to do, about)
+    // (those that have something to do, about: of a sequence's pieces one, so that its sums do not follow from how many there are)
+    const long blocks = p.n_kv_heads * (SHARED ? splits * ((p.n_tokens * p.group + 15) / 16) : items);
     MDMA_REQUIRE(items <= 65535 && p.n_kv_heads * splits <= 0x7fffffffl, "prefix_attention: grid too large");
     CUtensorMap mk, mv;
     if (int rc = prefix_cache_map(&mk, p.k_cache, p, kb)) return rc;
@@ -232,7 +233,8 @@ static int launch_prefix_stream(const PrefixParams& p, int sms, cudaStream_t str
         return 0;
     };
     // as many warps a block as leave every block resident at once, two at least (51 sequences x 32 kv heads, own keys and prefixes:
-    // 53 us in rounds of two-warp blocks, 56 with one warp, 67 with four)
+    // 53 us in rounds of two-warp blocks, 56 with one warp, 67 with four; a sequence of 30,000 own keys in 8 pieces beside four
+    // of 100, 8 kv heads: 61 us, with the warps for all pieces' blocks 98)
     const int nw = blocks <= sms ? 12 : blocks <= 3l * sms ? 4 : blocks <= 4l * sms ? 3 : 2;
 #define MDMA_STREAM(DM, KB) (nw == 12 ? run(prefix_stream_kernel<DM, KB, 12, SHARED>, 12, PoSmem<DM, KB, 12>::kBytes) \
                            : nw == 4 ? run(prefix_stream_kernel<DM, KB, 4, SHARED>, 4, PoSmem<DM, KB, 4>::kBytes) \

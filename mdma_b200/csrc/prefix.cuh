@@ -23,7 +23,7 @@ struct PrefixParams {
     int n_groups, n_seqs, n_tokens, max_new;
     int n_heads, n_kv_heads, head_dim, group;
     int pieces, own_splits;                          // a prefix in `pieces` pieces at most, own keys in `own_splits`: slots of the parts
-    int own_keys;                                    // of single tokens: keys of a piece of the own keys, the last takes the rest (0: equal pieces)
+    int own_keys;                                    // keys of a piece of streamed own keys, the last takes the rest (0: equal pieces)
     int unit;                                        // a piece of a prefix is a multiple of so many keys
     int whole;                                       // own_splits 0: all keys of a row tile, prefix and own ones, are one list in `pieces` pieces
     float scale_log2;                                // scale * log2(e)
@@ -42,7 +42,7 @@ __host__ __device__ __forceinline__ int prefix_pieces_used(int len, int pieces, 
     return (len + keys - 1) / keys;
 }
 
-// Piece `split` of a sequence's own keys [skip, end): keys [lo, hi), of a multiple of `unit`.  Pieces of a fixed length are the same
+// Piece `split` of a sequence's own keys [skip, end), of the streaming kernel: keys [lo, hi), of a multiple of `unit`.  Pieces of a fixed length are the same
 // whoever shares the step (only how many a step has room for follows from its longest sequence); most are empty beside one
 // long sequence.
 __device__ __forceinline__ void own_piece(const PrefixParams& p, int skip, int end, int split, int unit, int& lo, int& hi) {

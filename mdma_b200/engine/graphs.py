@@ -110,8 +110,6 @@ class DecodeSession:
         ctx.max_new, ctx.max_len = 1, self._bucket
         ctx.decode_only = True
         ctx.prefix = self.prefix
-        if self.prefix is not None:         # as `Engine.prefix_groups` bounds a step of its own
-            self.prefix.most_own = self._bucket - self.prefix.least_skip
         ctx.host_seq_new, ctx.host_seq_pos0, ctx.host_seq_slot = [1] * B, None, list(self.slots)
         return ctx
 
@@ -139,6 +137,10 @@ class DecodeSession:
         # to the bucket, so a graph stays valid until a sequence grows past it
         self._bucket = min(self.engine.max_context, -(-(longest + 1) // BUCKET) * BUCKET)
         n = max(1, min(n, self._bucket - longest))
+        if self.prefix is not None:             # the same for the keys behind shared prefixes (as `Engine.prefix_groups` bounds a step)
+            own = max(cache.length(s_) - skip for s_, skip in zip(self.slots, self.prefix.skips))
+            self.prefix.most_own = min(self.engine.max_context, -(-(own + 1) // BUCKET) * BUCKET)
+            n = max(1, min(n, self.prefix.most_own - own))
         while True:
             ext = {s: n for s in self.slots}
             why = cache.can_extend(ext)
@@ -161,7 +163,7 @@ class DecodeSession:
             if use_graph and self.graph_safe:
                 key = (B, self._bucket, draws)
                 if self.prefix is not None:       # what the grids and the tables' places follow from
-                    key += (self.prefix.n_groups, self.prefix.most_len, self.prefix.least_skip, self.prefix.n_shared, self.prefix.most_members)
+                    key += (self.prefix.n_groups, self.prefix.most_len, self.prefix.most_own, self.prefix.n_shared, self.prefix.most_members)
                 g = self.graphs.get(key)
                 if g is None:
                     # The first step at this batch size runs eagerly (it loads kernels); the same

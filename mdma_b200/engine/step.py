@@ -431,8 +431,7 @@ class Engine:
         groups = PrefixGroups(shared, pos0, new)
         if max(new) == 1:
             up = lambda n: min(self.max_context, -(-n // 1024) * 1024)  # noqa: E731
-            groups.most_len, groups.least_skip = up(groups.most_len), groups.least_skip // 1024 * 1024
-            groups.most_own = up(max(pos0) + 1) - groups.least_skip
+            groups.most_len, groups.most_own = up(groups.most_len), up(groups.most_own)
             groups.most_members = self.cache.most_members([slots[m] for _, members in shared for m in members])
         return groups
 

@@ -648,8 +648,12 @@ PREFIX_LEAST_BYTES = 100 << 20
 PREFIX_STREAM_ROWS = 24
 
 
-# Keys of a piece of the own keys of single tokens, at least, and what sequences x pieces may come to.
-PREFIX_OWN_KEYS = 1024
+# Keys of a piece of the own keys of single tokens, at least, where the engine's sequences fill the device (fewer in proportion where
+# they do not; multiples of 1,024), and what sequences x pieces may come to.  us of a call, 32/8 heads of 128, pieces of 1,024 / 2,048 /
+# 4,096 / 8,192 keys: one sequence of 30,000 own keys beside four behind 4,000 (32 slots) 61 / 61 / 61 / 86, uncut 219; four with
+# 8,000 own keys (32 slots) 53 / 53 / 49 / 70; sixteen with 8,000 (16 slots) 131 / 129 / 123 / 121; eight with 2,000 (8 slots) 49 / 45 /
+# 45 / 45.
+PREFIX_OWN_KEYS = 4096
 PREFIX_OWN_PARTS = 512
 
 
@@ -658,16 +662,19 @@ def prefix_streams(ctx, group: int, page_size: int) -> bool:
     return ctx.max_new == 1 and page_size % 32 == 0 and group <= 16 and ctx.n_tokens == ctx.n_seqs
 
 
-def prefix_own_cut(ctx, most_own: int) -> tuple[int, int]:
+def prefix_own_cut(ctx, most_own: int, n_kv_heads: int, sms: int) -> tuple[int, int]:
     """(pieces, keys of a piece) of the own keys of single tokens that are streamed: one block a (sequence, kv head) joins
     everything itself up to a piece's keys.  Keys beyond are cut into pieces of a fixed length, so that a step does not wait for the
-    one long sequence's blocks; the length, a multiple of 1,024, follows from the most sequences and the longest context that the
-    engine can hold.  Only their number follows from the live ones: a sequence's keys are cut at the same places, and its parts
+    one long sequence's blocks; their length follows from the most sequences and the longest context that the engine can hold.  Only their number follows from the live ones: a sequence's keys are cut at the same places, and its parts
     joined in the same order, whoever shares the step."""
-    seqs = getattr(ctx, "most_seqs", None) or ctx.n_seqs
+    return _own_cut(getattr(ctx, "most_seqs", None) or ctx.n_seqs, max(most_own, getattr(ctx, "most_len", None) or 0), most_own, n_kv_heads, sms,
+                    PREFIX_OWN_KEYS // 4)
+
+
+@functools.lru_cache(maxsize=4096)
+def _own_cut(seqs: int, longest: int, most_own: int, n_kv_heads: int, sms: int, unit: int) -> tuple[int, int]:
     most = max(1, min(PREFIX_OWN_PARTS // seqs, 16))
-    longest = max(most_own, getattr(ctx, "most_len", None) or 0)
-    keys = -(-longest // (most * PREFIX_OWN_KEYS)) * PREFIX_OWN_KEYS
+    keys = unit * max(min(4, -(-4 * seqs * n_kv_heads // sms)), -(-longest // (most * unit)))
     return max(1, min(most, -(-most_own // keys))), keys
 
 
@@ -695,22 +702,26 @@ def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, 
     one list in n pieces; (0, n, ..): every sequence reads its prefix by itself."""
     one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
-    streams = prefix_streams(ctx, group, page_size)
+    streams = one and prefix_streams(ctx, group, page_size)
     if streams and seqs * g.most_len * n_kv_heads * head_dim * 4 <= PREFIX_LEAST_BYTES:
-        return 0, prefix_own_cut(ctx, g.most_len + g.most_own)[0], PREFIX_STREAM
-    most_own = max(g.most_own, getattr(ctx, "most_len", None) or 0) if one else g.most_own
-    pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, most_own, n_heads, n_kv_heads)
-    if streams:
-        own = prefix_own_cut(ctx, g.most_own)[0]
+        # (equal pieces of every sequence, unless the blocks cover the device or have less than a thousand keys each)
+        keys, blocks = g.most_len + g.most_own, seqs * n_kv_heads
+        return 0, 1 if 2 * blocks > sms or keys <= 1024 else max(1, min(sms // blocks, keys // 512, 16)), PREFIX_STREAM
     rows, shared = group * (getattr(g, "most_members", None) or g.most_tokens), getattr(g, "n_shared", None) or g.n_groups
     if streams and (rows <= PREFIX_STREAM_ROWS or page_size % 64):
         tiles = -(-seqs // (16 // group)) * n_kv_heads
-        return max(1, min(2 * sms // tiles, 32, -(-g.most_len // 256))), own, PREFIX_STREAM
-    if page_size % 64 == 0:                       # 256 query rows a block, one block an SM
-        tile_tokens = 2 * (128 // group)
-        tiles = max(shared, -(-seqs // tile_tokens)) if one else ctx.n_tokens // tile_tokens + g.n_groups
-        if not one:
-            return max(1, min(sms // (tiles * n_kv_heads), 32, (g.most_len + g.most_own) // 256)), 0, PREFIX_TC
+        return max(1, min(2 * sms // tiles, 32, -(-g.most_len // 256))), prefix_own_cut(ctx, g.most_own, n_kv_heads, sms)[0], PREFIX_STREAM
+    tile_tokens = 2 * (128 // group)              # of the tcgen05 kernel: 256 query rows a block, one block an SM
+    if not one and page_size % 64 == 0:
+        tiles = ctx.n_tokens // tile_tokens + g.n_groups
+        return max(1, min(sms // (tiles * n_kv_heads), 32, (g.most_len + g.most_own) // 256)), 0, PREFIX_TC
+    if streams:
+        own = prefix_own_cut(ctx, g.most_own, n_kv_heads, sms)[0]
+    else:
+        most_own = max(g.most_own, getattr(ctx, "most_len", None) or 0) if one else g.most_own
+        pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, most_own, n_heads, n_kv_heads)
+    if page_size % 64 == 0:
+        tiles = max(shared, -(-seqs // tile_tokens))
         return _tc_pieces(tiles * n_kv_heads, -(-g.most_len // 128), prefix_tc_pieces(seqs, group, n_kv_heads, sms), sms), own, PREFIX_TC
     return pieces, own, PREFIX_ROWS
 
@@ -731,9 +742,7 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     flush_pending(q.device, st)
     g = ctx.prefix
     pieces, own, kind = prefix_plan(ctx, g, n_heads, n_kv_heads, head_dim, st.sms, view.page_size)
-    own_keys = 0
-    if own > 0 and prefix_streams(ctx, n_heads // n_kv_heads, view.page_size):
-        own_keys = prefix_own_cut(ctx, g.most_own + (0 if pieces else g.most_len))[1]
+    own_keys = prefix_own_cut(ctx, g.most_own, n_kv_heads, st.sms)[1] if pieces and own and ctx.max_new == 1 else 0
     need = ops.prefix_scratch_floats(ctx.n_tokens, n_heads, pieces + own, head_dim) if pieces + own > 1 else 0
     if own_st is not None:
         st.need(need, "attention over shared prefixes")

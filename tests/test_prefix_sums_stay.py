@@ -71,13 +71,13 @@ def test_the_length_of_a_piece_follows_from_the_engine(most_seqs, most_len):
     lengths = set()
     for live in (1, 2, most_seqs):
         for own in (1, 20, 1024, 1025, most_len // 2 + 1, most_len):
-            pieces, keys = ops_tensor.prefix_own_cut(meta(live, most_seqs, most_len), min(own, most_len))
+            pieces, keys = ops_tensor.prefix_own_cut(meta(live, most_seqs, most_len), min(own, most_len), 8, 148)
             lengths.add(keys)
             assert 1 <= pieces <= 16 and pieces * keys >= min(own, most_len) and (pieces - 1) * keys < own
             assert pieces * most_seqs <= max(most_seqs, ops_tensor.PREFIX_OWN_PARTS)
     assert len(lengths) == 1 and lengths.pop() % 1024 == 0
     if most_seqs <= 64 and most_len == 32768:
-        assert ops_tensor.prefix_own_cut(meta(5, most_seqs, most_len), 30000)[0] >= 7
+        assert ops_tensor.prefix_own_cut(meta(5, most_seqs, most_len), 30000, 8, 148)[0] >= 7
 
 
 @pytest.mark.parametrize("heads, kv_heads, page", [(32, 8, 64), (32, 32, 64), (64, 2, 64), (8, 2, 16), (8, 8, 32)])
@@ -95,23 +95,24 @@ def test_plans_do_not_follow_from_the_longest_sequence(heads, kv_heads, page):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", [0, 1], ids=["tcgen05", "streamed"])
-@pytest.mark.parametrize("shared", [True, False], ids=["", "alone"])
-def test_pieces_of_a_fixed_length(kind, shared, monkeypatch):
+def test_pieces_of_a_fixed_length(kind, monkeypatch):
     """Against the definition in pieces of 128 keys; bit for bit the same whether a step has room for the pieces of its longest sequence,
     or for many more; and right if it has been given too few."""
-    monkeypatch.setattr(ops_tensor, "PREFIX_OWN_KEYS", 128)
+    monkeypatch.setattr(ops_tensor, "PREFIX_OWN_KEYS", 512)
     ctx, q, view, dense = make_batch([(200, [(0, 1), (127, 1), (128, 1), (1, 1)]), (0, [(500, 1), (5, 1)])], 8, 2, 64, 64, torch.bfloat16, 4, "cuda")
     ref = definition(ctx, q, dense, 8, 2, 64, 0.125)
+    ctx.most_seqs = 16                                # (their 32 blocks: pieces of a quarter)
     outs, longest = [], ctx.prefix.most_own
-    for most_own, most_len in ((longest, 0), (longest + 300, 0), (40, 0), (40, 900)):
-        ctx.prefix.most_own, ctx.most_seqs, ctx.most_len = most_own, 32, most_len
-        plan = (3 if shared else 0, ops_tensor.prefix_own_cut(ctx, most_own + (0 if shared else 200))[0], kind if shared else 1)
-        monkeypatch.setattr(ops_tensor, "prefix_plan", lambda *a: plan)
+    for most_own in (longest, longest + 300, 40):
+        ctx.prefix.most_own = most_own
+        own, keys = ops_tensor.prefix_own_cut(ctx, most_own, 2, 148)
+        assert keys == 128 and own == {longest: 4, longest + 300: 7, 40: 1}[most_own]
+        monkeypatch.setattr(ops_tensor, "prefix_plan", lambda *a: (3, own, kind))
         out = torch.empty(ctx.n_tokens, 512, dtype=torch.bfloat16, device="cuda")
         ops_tensor.prefix_attention(ctx, q, view, out, 8, 2, 64, 0.125)
         ops_tensor.check_status(q.device)
-        check_close(out, ref, 64, torch.bfloat16, f"{plan}")
+        check_close(out, ref, 64, torch.bfloat16, f"{own} pieces")
         outs.append(out)
     assert torch.equal(outs[0], outs[1])
-    short = [i for i in range(ctx.n_seqs) if int(ctx.seq_pos0[i]) + 1 - (int(ctx.prefix.seq_skip[i]) if shared else 0) <= 128]
-    assert len(short) >= (4 if shared else 1) and all(torch.equal(outs[0][short], o[short]) for o in outs[1:])
+    short = [i for i in range(ctx.n_seqs) if int(ctx.seq_pos0[i]) + 1 - int(ctx.prefix.seq_skip[i]) <= 128]
+    assert len(short) == 4 and torch.equal(outs[0][short], outs[2][short])
