@@ -84,10 +84,11 @@ class Layout:
 
 def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max_tokens: int, max_slots: int,
             max_context: int, page_size: int, chunk_tokens: int, logit_rows: int, history_cap: int,
-            run_ahead: int = 8, stored: Optional[dict] = None) -> Layout:
+            run_ahead: int = 8, stored: Optional[dict] = None, shares: bool = True) -> Layout:
     """Carve the engine's memory, in a fixed order: weights, cache, workspace, logits, step
     metadata, sampler, kernel scratch, tables the parts derive.  Run with a planning carver this
-    is the memory plan (src/model/planning.rs:55-125); run over the arena it is the allocation."""
+    is the memory plan (src/model/planning.rs:55-125); run over the arena it is the allocation.
+    `shares`: with room for steps that read shared prefixes once (without it forks read sequence by sequence)."""
     from ..sampling.sampler import DeviceSampler
     lay = Layout()
     expected = model.expected_tensors()
@@ -103,14 +104,14 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
         lay.workspace[name] = carver.take("workspace", (chunk_tokens, cols), dt)
     lay.logits = carver.take("logits", (logit_rows, model.spec.vocab_size), torch.float32)
     # (ids, positions, .. of a pass, and who shares what)
-    lay.meta_cap = 6 * chunk_tokens + 4 * max_slots + logit_rows + 16 + chunk_tokens + 4 * max_slots + 1
+    lay.meta_cap = 6 * chunk_tokens + 4 * max_slots + logit_rows + 16 + (chunk_tokens + 4 * max_slots + 1 if shares else 0)
     lay.meta_dev = carver.take("metadata", (lay.meta_cap,), torch.int32)
     # the replayed decode step reads its inputs from here: ids, positions (twice), slots, 0..cap
     # (the first four side by side: one copy brings them)
     rows = carver.take("metadata", (4, max_slots), torch.int32)
     lay.decode = {name: rows[i] if rows is not None else None for i, name in enumerate(("ids", "tok_pos", "seq_slot", "seq_pos0"))}
     lay.decode["rows"] = rows
-    lay.decode["prefix"] = carver.take("metadata", (5 * max_slots + 1,), torch.int32)
+    lay.decode["prefix"] = carver.take("metadata", (5 * max_slots + 1,), torch.int32) if shares else None
     lay.decode["arange"] = carver.take("metadata", (max_slots + 1,), torch.int32)
     lay.sampler = DeviceSampler(model.spec.vocab_size, max_slots, device, history_cap, alloc=carver.taker("sampler"))
     # the result words (tokens, flags, status) of the last `run_ahead` replayed decode steps
@@ -127,7 +128,8 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
     if dtype == torch.bfloat16:
         from .. import ops_tensor
         floats = ops_tensor.scratch_floats_bound(sms, chunk_tokens, max_slots, shapes)
-    floats = max(floats, prefix_floats(model, dtype, sms, max_slots, max_context, page_size))
+    if shares:
+        floats = max(floats, prefix_floats(model, dtype, sms, max_slots, max_context, page_size))
     lay.scratch_floats = floats
     lay.tc_sk_flags = carver.take("kernel_scratch", (max(512, 4 * sms),), torch.int32)
     lay.tc_scratch = carver.take("kernel_scratch", (max(floats, 1),), torch.float32)
@@ -264,14 +266,19 @@ class Engine:
                      max_slots=self.max_slots, max_context=self.max_context, page_size=page_size,
                      chunk_tokens=self.chunk_tokens, logit_rows=self.logit_rows, history_cap=history_cap,
                      run_ahead=run_ahead, stored=stored)
-        planner = Carver()
-        planned = lay_out(self.model, planner, **sizes)
-        self.plan = _plan_dict(planner, planned.cache, page_size, self.max_slots, self.chunk_tokens, self.logit_rows)
         free, _total = torch.cuda.mem_get_info(self.device)
         if vram_bytes is not None:
             free = min(free, int(vram_bytes))
-        need = self.plan["total_bytes"] + reserve_mib * (1 << 20)
-        if need > free:
+        # (a budget that does without what reads shared prefixes once is not refused for it)
+        for self.reads_shared in (True, False):
+            sizes["shares"] = self.reads_shared
+            planner = Carver()
+            planned = lay_out(self.model, planner, **sizes)
+            self.plan = _plan_dict(planner, planned.cache, page_size, self.max_slots, self.chunk_tokens, self.logit_rows)
+            need = self.plan["total_bytes"] + reserve_mib * (1 << 20)
+            if need <= free:
+                break
+        else:
             raise MemoryBudgetError(need, free, self.plan)
 
         with torch.cuda.device(self.device):
@@ -425,7 +432,7 @@ class Engine:
         multiples of 1,024 as the replayed graphs see them (a graph serves every batch within its bounds), so that a step on
         its own adds up in the same order."""
         shared = [(length, members) for length, members in self.cache.shared_prefixes(slots)
-                  if all(pos0[m] >= length for m in members)]
+                  if all(pos0[m] >= length for m in members)] if self.reads_shared else []
         if not shared:
             return None
         groups = PrefixGroups(shared, pos0, new)

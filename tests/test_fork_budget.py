@@ -1,0 +1,45 @@
+"""Engines whose budget holds everything but the room for shared prefixes: they are built, and their forks read sequence by sequence."""
+import numpy as np
+import pytest
+import torch
+
+from replay_util import TOL_F32
+from test_forks import ids, step
+from tiny import SHARP, TINY_A, TINY_D, make_model
+
+
+def engine(d, dtype, **budget):
+    from mdma_b200.engine import Engine
+    return Engine(d, dtype=dtype, max_batch=6, max_context=256, reserve_mib=0, **budget)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cfg", [TINY_A, TINY_D], ids="AD")
+def test_a_budget_without_room_for_shared_prefixes(cfg):
+    from mdma_b200.engine import MemoryBudgetError
+    d, _, _ = make_model(cfg, 2, torch.float32, std_scale=SHARP)
+    whole = engine(d, "float32")
+    most = whole.memory_plan()["total_bytes"]
+    small = engine(d, "float32", vram_bytes=most - 1)
+    plan = small.memory_plan()
+    assert plan["total_bytes"] < most and small.held_bytes()["total_bytes"] == plan["total_bytes"]
+    assert plan["kernel_scratch_bytes"] < whole.memory_plan()["kernel_scratch_bytes"]
+    with pytest.raises(MemoryBudgetError) as e:
+        engine(d, "float32", vram_bytes=plan["total_bytes"] - 1)
+    assert e.value.requested == plan["total_bytes"]
+    got = []
+    for eng in (whole, small):
+        a = eng.acquire()
+        step(eng, [(a, ids(cfg, 100, 0))])
+        slots = [a] + eng.fork(a, 3)
+        rows = [step(eng, [(s, ids(cfg, 3, i), [2]) for i, s in enumerate(slots)]),
+                step(eng, [(s, [5 + j], [0]) for j, s in enumerate(slots)])]
+        session = eng.decode_session()
+        session.start(slots, [3] * 4)
+        session.run(1)
+        rows.append(session.logits[:4].double().cpu().numpy())
+        got.append(np.concatenate(rows))
+        assert (eng.prefix_groups(slots, [110] * 4, [1] * 4) is None) == (eng is small)
+    assert np.abs(got[0] - got[1]).max() <= 2 * TOL_F32 * max(1.0, np.abs(got[0]).max())
+    outs = [eng.generate([ids(cfg, 40, 7)], max_tokens=8, n=2)[1].tokens for eng in (whole, small)]
+    assert outs[0] == outs[1] and len(outs[0]) == 8
