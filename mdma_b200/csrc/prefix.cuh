@@ -21,6 +21,7 @@ struct PrefixParams {
     void* out;
     float* part_o; float* part_ml;                   // [token][head][slot][head_dim], [token][head][slot][2]
     int n_groups, n_seqs, n_tokens, max_new;
+    int n_shared;                                    // groups that have a prefix, at most
     int n_heads, n_kv_heads, head_dim, group;
     int pieces, own_splits;                          // a prefix in `pieces` pieces at most, own keys in `own_splits`: slots of the parts
     int own_keys;                                    // keys of a piece of streamed own keys, the last takes the rest (0: equal pieces)
@@ -84,9 +85,11 @@ __device__ __forceinline__ bool prefix_tile(const PrefixParams& p, int t, int ti
     }
     return false;
 }
-// The most tiles a step can have: every group leaves one partly filled.
+// The most tiles a step can have: every group leaves one partly filled.  (Sequences that share nothing are groups, too, but have
+// no tiles unless their own keys are walked: with a block for each, 8 sequences behind 2,048 tokens beside 56 that share
+// nothing took 108 us on the tcgen05 kernel, whose blocks do not share an SM.)
 static inline long prefix_tiles_bound(const PrefixParams& p, int tile_tokens) {
-    return (long)p.n_tokens / tile_tokens + p.n_groups;
+    return (long)p.n_tokens / tile_tokens + (p.whole ? p.n_groups : p.n_shared);
 }
 
 // A part's share of the whole, 2^(its maximum - m).  -1, no share: a part without keys leaves no maximum and no sum.  (The
@@ -152,7 +155,7 @@ static inline unsigned prefix_merge_blocks(const PrefixParams& p) {
 // The arguments as one array of 64-bit words, in the order below (a step makes this call once a layer: converting thirty
 // arguments one by one costs the host more than the launches).
 static inline int prefix_params(const long long* w, int n_words, float scale, PrefixParams* out) {
-    MDMA_REQUIRE(n_words == 33, "prefix_attention: %d argument words", n_words);
+    MDMA_REQUIRE(n_words == 34, "prefix_attention: %d argument words", n_words);
     PrefixParams& p = *out;
     int i = 0;
     auto ptr = [&]() { return (void*)(uintptr_t)w[i++]; };
@@ -166,7 +169,7 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     p.out = ptr();
     float* scratch = (float*)ptr();
     const long long floats = w[i++];
-    p.n_groups = num(); p.n_seqs = num(); p.n_tokens = num(); p.max_new = num();
+    p.n_groups = num(); p.n_shared = num(); p.n_seqs = num(); p.n_tokens = num(); p.max_new = num();
     p.n_heads = num(); p.n_kv_heads = num(); p.head_dim = num();
     p.pieces = num(); p.own_splits = num(); p.own_keys = num();
     p.sinks = (const float*)ptr();
@@ -176,7 +179,7 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     MDMA_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0, "prefix_attention: %d heads over %d kv heads", p.n_heads, p.n_kv_heads);
     MDMA_REQUIRE(p.head_dim > 0 && p.head_dim <= 256, "prefix_attention: head_dim %d is beyond the limit of 256", p.head_dim);
     MDMA_REQUIRE(p.page_table && p.page_size > 0 && p.max_pages > 0, "prefix_attention: bad cache geometry");
-    MDMA_REQUIRE(p.n_groups >= 0 && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 0 && p.own_splits >= 0 && p.own_keys >= 0 && p.pieces + p.own_splits > 0, "prefix_attention: bad sizes");
+    MDMA_REQUIRE(p.n_groups >= 0 && p.n_shared >= 0 && p.n_shared <= p.n_groups && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 0 && p.own_splits >= 0 && p.own_keys >= 0 && p.pieces + p.own_splits > 0, "prefix_attention: bad sizes");
     MDMA_REQUIRE(p.pieces <= 32 && p.own_splits <= 32, "prefix_attention: %d and %d pieces are beyond the limit of 32", p.pieces, p.own_splits);
     MDMA_REQUIRE(scale > 0.f, "prefix_attention: the score scale must be positive");
     p.group = p.n_heads / p.n_kv_heads;

@@ -1219,9 +1219,10 @@ def prefix_words(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int
         q.data_ptr(), q.stride(0), view.k.data_ptr(), view.v.data_ptr(), ctx.seq_start.data_ptr(), ctx.seq_pos0.data_ptr(),
         ctx.seq_slot.data_ptr(), ctx.tok_seq.data_ptr(), view.page_table.data_ptr(), view.max_pages, view.page_size,
         view.k.size(0), g.group_len.data_ptr(), g.group_seq.data_ptr(), g.tok_first.data_ptr(), g.toks.data_ptr(),
-        g.seq_skip.data_ptr(), out.data_ptr(), scratch.data_ptr(), scratch.numel(), g.n_groups, ctx.n_seqs, ctx.n_tokens,
-        ctx.max_new, n_heads, n_kv_heads, head_dim, pieces, own_splits, own_keys, 0 if sinks is None else sinks.data_ptr(),
-        0 if status is None else status.data_ptr(), int(sinks_log2)))
+        g.seq_skip.data_ptr(), out.data_ptr(), scratch.data_ptr(), scratch.numel(), g.n_groups,
+        getattr(g, "n_shared", None) or g.n_groups, ctx.n_seqs, ctx.n_tokens, ctx.max_new, n_heads, n_kv_heads, head_dim,
+        pieces, own_splits, own_keys, 0 if sinks is None else sinks.data_ptr(), 0 if status is None else status.data_ptr(),
+        int(sinks_log2)))
 
 
 def prefix_checks(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: int, sinks) -> None:

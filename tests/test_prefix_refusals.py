@@ -4,7 +4,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from prefix_util import make_batch
+from prefix_util import check_close, definition, make_batch
 from mdma_b200 import ops, ops_tensor
 from mdma_b200.ops import KernelError
 
@@ -30,3 +30,27 @@ def test_tables_of_another_layout(fn):
     assert (out == 7.0).all()
     fn(ctx, q, view, out, 8, 2, 64, 0.125)
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", ["float32", "bfloat16", "tcgen05", "streamed", "whole lists"])
+def test_few_families_among_many_that_share_nothing(path, monkeypatch):
+    """The grid has room for the families' tiles, wherever they stand among the groups, and not for a tile a sequence."""
+    dtype = torch.float32 if path == "float32" else torch.bfloat16
+    new = 3 if path == "whole lists" else 1
+    groups = [(0, [(i % 7, new)]) for i in range(40)] + [(100, [(i, new) for i in range(9)])] + [(0, [(70, new)])] + [(65, [(0, new)])] + [(200, [(3, new)] * 30)]
+    ctx, q, view, dense = make_batch(groups, 8, 2, 64, 64, dtype, 3, "cuda")
+    assert ctx.prefix.n_groups == 44 and ctx.prefix.n_shared == 3
+    if path in ("tcgen05", "streamed"):
+        monkeypatch.setattr(ops_tensor, "prefix_plan", lambda *a: (2, 1, 0 if path == "tcgen05" else 1))
+    order = torch.randperm(44, generator=torch.Generator().manual_seed(1)).tolist()          # families first, last and in between
+    host = ctx.prefix._host
+    firsts = host["tok_first"].tolist()
+    toks = [host["toks"][firsts[g]:firsts[g + 1]] for g in order]
+    ints = lambda x: torch.tensor([int(n) for n in x], dtype=torch.int32, device="cuda")  # noqa: E731
+    ctx.prefix.group_len, ctx.prefix.group_seq = ints(host["group_len"][g] for g in order), ints(host["group_seq"][g] for g in order)
+    ctx.prefix.toks = ints(t for part in toks for t in part)
+    ctx.prefix.tok_first = ints([0] + [sum(len(p) for p in toks[:i + 1]) for i in range(44)])
+    out = torch.empty(ctx.n_tokens, 512, dtype=dtype, device="cuda")
+    (ops if path in ("float32", "bfloat16") else ops_tensor).prefix_attention(ctx, q, view, out, 8, 2, 64, 0.125)
+    check_close(out, definition(ctx, q, dense, 8, 2, 64, 0.125), 64, dtype)
