@@ -334,6 +334,10 @@ class SequenceCache:
         """The most sequences that have shared a fork of one of these at a time (who has ended counts on while another is left)."""
         return max((self.families[self.shares[s][0]] for s in slots if s in self.shares), default=0)
 
+    def shared_keys(self, slots) -> int:
+        """The tokens that these sequences' forks share, each as often as sequences have shared it at a time (as `most_members`)."""
+        return sum(length * self.families[fork] for fork, length in {self.shares[s] for s in slots if s in self.shares})
+
     def compact(self) -> int:
         """Move held pages from the rear of each group's pool to free ones at its front, so that the held pages are the pool's
         first; returns how many were moved.  Tables follow; what is shared stays shared."""

@@ -44,9 +44,11 @@ class PrefixGroups:
         toks = [np.arange(starts[m], starts[m + 1]) for _, members in groups for m in members]
         sizes = [int(sum(starts[m + 1] - starts[m] for m in members)) for _, members in groups]
         self.n_groups = len(groups)
-        # what plans go by: groups with a prefix, the members of the largest (an engine counts those that have ended, too)
+        # what plans go by: groups with a prefix, the members of the largest, the keys that all members see of their prefixes (an
+        # engine counts those that have ended, too)
         self.n_shared = sum(1 for length, _ in groups if length)
         self.most_members = max((len(members) for length, members in groups if length), default=0)
+        self.shared_keys = sum(length * len(members) for length, members in groups)
         self.most_tokens = max(sizes, default=0)
         self.most_len = max((length for length, _ in groups), default=0)
         self.skips = skip

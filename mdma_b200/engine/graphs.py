@@ -163,7 +163,8 @@ class DecodeSession:
             if use_graph and self.graph_safe:
                 key = (B, self._bucket, draws)
                 if self.prefix is not None:       # what the grids and the tables' places follow from
-                    key += (self.prefix.n_groups, self.prefix.most_len, self.prefix.most_own, self.prefix.n_shared, self.prefix.most_members)
+                    g = self.prefix
+                    key += (g.n_groups, g.most_len, g.most_own, g.n_shared, g.most_members, g.shared_keys)
                 g = self.graphs.get(key)
                 if g is None:
                     # The first step at this batch size runs eagerly (it loads kernels); the same

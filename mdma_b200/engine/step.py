@@ -150,10 +150,10 @@ def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_cont
         for heads, kv_heads, head_dim in getattr(part, "prefix_shapes", list)():
             parts = sum(ops.prefix_plan(ctx, most, heads, kv_heads))
             if dtype == torch.bfloat16 and ops_tensor.attention_supported(heads, kv_heads, head_dim):
-                for most.most_members in (1, max_slots):       # (fewer families or more: at most `prefix_tc_pieces`)
+                for most.most_members in (1, max_slots):       # (fewer families or more: at most `prefix_most_pieces`)
                     pieces, own, kind = ops_tensor.prefix_plan(ctx, most, heads, kv_heads, head_dim, sms, page_size)
-                    if kind == ops_tensor.PREFIX_TC:
-                        pieces = ops_tensor.prefix_tc_pieces(max_slots, heads // kv_heads, kv_heads, sms)
+                    if kind != ops_tensor.PREFIX_ROWS:
+                        pieces = max(pieces, ops_tensor.prefix_most_pieces(max_slots, heads // kv_heads, kv_heads, sms))
                     parts = max(parts, pieces + own)
             need = max(need, ops.prefix_scratch_floats(min(max_slots, 512), heads, parts, head_dim))
     return need
@@ -439,7 +439,12 @@ class Engine:
         if max(new) == 1:
             up = lambda n: min(self.max_context, -(-n // 1024) * 1024)  # noqa: E731
             groups.most_len, groups.most_own = up(groups.most_len), up(groups.most_own)
-            groups.most_members = self.cache.most_members([slots[m] for _, members in shared for m in members])
+            those = [slots[m] for _, members in shared for m in members]
+            groups.most_members = self.cache.most_members(those)
+            if groups.most_len <= 1024:          # (what plans of short prefixes go by; to a power of two, for few graphs)
+                groups.shared_keys = 1 << max(10, (self.cache.shared_keys(those) - 1).bit_length())
+            else:
+                groups.shared_keys = 0
         return groups
 
     # ---- the step ----------------------------------------------------------

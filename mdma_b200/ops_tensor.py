@@ -638,13 +638,18 @@ def attention_general(ctx, q: torch.Tensor, view, n_heads: int, n_kv_heads: int,
 
 
 # ---- attention of sequences that share their beginning (csrc/attention_prefix.cu) ------------------------------------------
-# Prefix bytes times sequences up to which every sequence of a single-token step reads its prefix by itself, and the query rows
-# of a kv head in the largest family up to which prefixes are streamed.  us, alone / streamed / tcgen05, heads of 128:
-# 4 sequences behind 300 tokens, 32/8 heads of 64: 5.5 / 11; 8 behind 2,048, 32/8 (64 MiB, 32 rows): 16.1 / 14.5 / 18.0;
-# 16 behind 2,048, 32/8 (128 MiB, 64 rows): 20.9 / 18.7 / 18.7; 16 behind 2,048, 32/32 (16 rows): 69 / 25.5 / 29.9;
-# 4 families of 6 behind 2,000, 32/8 (24 rows): - / 20.4 / 24.0; 6 of 8 behind 6,000, 32/8 (32 rows): 135 / 55.7 / 49.7;
-# 32 behind 16,000, 32/32 (32 rows): 1,016 / 111 / 86.
+# Bytes of keys and values up to which every sequence of a single-token step reads its prefix by itself: the longest prefix for as
+# many sequences as the engine can hold; of prefixes up to PREFIX_SHORT tokens what the families have in common.  And the query rows of a
+# kv head in the largest family up to which prefixes are streamed.  us of a layer in a replayed decode step (width 4,096, feed-forward
+# 1,024, products and norms with it), by itself / streamed / tcgen05; heads of 128, own keys 20, sequences that share nothing hold 500:
+#   32/8 heads, 8 behind 2,048, 8 slots 70 / 73 / 80; 8 behind 8,192 94 / 82 / 87; 2 behind 8,192, 2 slots 69 / 81 / 84;
+#   64 slots: 2 behind 20 beside 62 103 / 110 / 116; 2 behind 2,048 beside 62 142 / 112 / 120; 8 behind 512 beside 56 101 / 116 / 125;
+#   8 behind 2,048 beside 56 145 / 122 / 120; 4 behind 500 61 / 67 / 74; 4 behind 8,192 80 / 78 / 88; 16 behind 2,048 81 / 76 / 81;
+#   16 behind 8,192 126 / 93 / 87; 64 behind 512 97 / 99 / 105; 64 behind 1,000 113 / 105 / 105;
+#   32/32 heads, 64 slots: 2 behind 2,048 74 / 83 / 92, beside 62 220 / 188 / 199; 16 behind 2,048 127 / 87 / 95; 64 behind 512 173 / 121 / 126.
+# (The borders are not the best one everywhere: what they miss here is up to 9 us, 64 behind 512 and two behind 2,048 with 32 kv heads.)
 PREFIX_LEAST_BYTES = 100 << 20
+PREFIX_SHORT = 1024
 PREFIX_STREAM_ROWS = 24
 
 
@@ -682,8 +687,8 @@ def _own_cut(seqs: int, longest: int, most_own: int, n_kv_heads: int, sms: int, 
 PREFIX_TC, PREFIX_STREAM, PREFIX_ROWS = 0, 1, 2
 
 
-def prefix_tc_pieces(seqs: int, group: int, n_kv_heads: int, sms: int) -> int:
-    """The most pieces of a prefix that the tcgen05 kernel cuts it into for single tokens of up to so many sequences."""
+def prefix_most_pieces(seqs: int, group: int, n_kv_heads: int, sms: int) -> int:
+    """The most pieces that few families' prefixes are cut into for single tokens of up to so many sequences."""
     return min(32, max(4, sms // (-(-seqs // (2 * (128 // group))) * n_kv_heads)))
 
 
@@ -703,14 +708,19 @@ def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, 
     one, group = ctx.max_new == 1, n_heads // n_kv_heads
     seqs = (getattr(ctx, "most_seqs", None) or ctx.n_seqs) if one else ctx.n_seqs
     streams = one and prefix_streams(ctx, group, page_size)
-    if streams and seqs * g.most_len * n_kv_heads * head_dim * 4 <= PREFIX_LEAST_BYTES:
+    keys = seqs * g.most_len
+    if g.most_len <= PREFIX_SHORT:
+        keys = getattr(g, "shared_keys", 0) or keys
+    if streams and keys * n_kv_heads * head_dim * 4 <= PREFIX_LEAST_BYTES:
         # (equal pieces of every sequence, unless the blocks cover the device or have less than a thousand keys each)
         keys, blocks = g.most_len + g.most_own, seqs * n_kv_heads
         return 0, 1 if 2 * blocks > sms or keys <= 1024 else max(1, min(sms // blocks, keys // 512, 16)), PREFIX_STREAM
     rows, shared = group * (getattr(g, "most_members", None) or g.most_tokens), getattr(g, "n_shared", None) or g.n_groups
     if streams and (rows <= PREFIX_STREAM_ROWS or page_size % 64):
-        tiles = -(-seqs // (16 // group)) * n_kv_heads
-        return max(1, min(2 * sms // tiles, 32, -(-g.most_len // 256))), prefix_own_cut(ctx, g.most_own, n_kv_heads, sms)[0], PREFIX_STREAM
+        each = 16 // group                        # tokens a tile
+        pieces = max(min(2 * sms // (-(-seqs // each) * n_kv_heads), 32),
+                     min(2 * sms // (shared * -(-rows // (group * each)) * n_kv_heads), prefix_most_pieces(seqs, group, n_kv_heads, sms)))
+        return max(1, min(pieces, -(-g.most_len // 256))), prefix_own_cut(ctx, g.most_own, n_kv_heads, sms)[0], PREFIX_STREAM
     tile_tokens = 2 * (128 // group)              # of the tcgen05 kernel: 256 query rows a block, one block an SM
     if not one and page_size % 64 == 0:
         tiles = ctx.n_tokens // tile_tokens + g.n_groups
@@ -722,7 +732,7 @@ def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, 
         pieces, own = ops.prefix_split(64, 2 * sms, seqs if one else ctx.n_tokens, seqs, ctx.max_new, g.most_len, most_own, n_heads, n_kv_heads)
     if page_size % 64 == 0:
         tiles = max(shared, -(-seqs // tile_tokens))
-        return _tc_pieces(tiles * n_kv_heads, -(-g.most_len // 128), prefix_tc_pieces(seqs, group, n_kv_heads, sms), sms), own, PREFIX_TC
+        return _tc_pieces(tiles * n_kv_heads, -(-g.most_len // 128), prefix_most_pieces(seqs, group, n_kv_heads, sms), sms), own, PREFIX_TC
     return pieces, own, PREFIX_ROWS
 
 
