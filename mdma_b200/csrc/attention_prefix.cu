@@ -17,7 +17,7 @@ constexpr int kPrRows = 64, kPrKeys = 64, kPrThreads = 128;
 // the merge.
 template <int DMAX>
 __global__ void __launch_bounds__(kPrThreads)
-prefix_rows_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
+prefix_rows_kernel(const PrefixParams p, int own_tiles) {           // own_tiles: of a sequence; 0: the prefixes
     constexpr int kChunks = DMAX / 8, kTile = kPrRows * DMAX * 2;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int row_token[kPrRows];
@@ -28,19 +28,19 @@ prefix_rows_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
     chain_release();
     const int G = p.group, D = p.head_dim, kvh = blockIdx.y, tt = kPrRows / G, split = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool prefix = (int)blockIdx.x < prefix_tiles;
+    const bool prefix = own_tiles == 0;
     int lo, hi, slot, n_tok, seq, first_pos = 0;     // keys [lo, hi); the tile's tokens stand at first_pos, first_pos + 1, ..
     if (prefix) {
         PrefixTile t;
-        if (split >= p.pieces || !prefix_tile(p, blockIdx.x, tt, t)) return;
+        if (!prefix_tile(p, blockIdx.x, tt, t)) return;
         const int len = p.group_len[t.g], keys = prefix_piece(len, p.pieces, p.unit);
         lo = split * keys; hi = min(len, lo + keys); slot = split; n_tok = t.count; seq = p.group_seq[t.g];
         if (lo >= hi) return;
         if ((int)threadIdx.x < kPrRows) row_token[threadIdx.x] = (int)threadIdx.x / G < n_tok ? p.toks[t.first + threadIdx.x / G] : -1;
     } else {
-        seq = ((int)blockIdx.x - prefix_tiles) / own_tiles;
-        const int tok0 = ((int)blockIdx.x - prefix_tiles) % own_tiles * tt, n_new = p.seq_start[seq + 1] - p.seq_start[seq];
-        if (split >= p.own_splits || tok0 >= n_new) return;
+        seq = (int)blockIdx.x / own_tiles;
+        const int tok0 = (int)blockIdx.x % own_tiles * tt, n_new = p.seq_start[seq + 1] - p.seq_start[seq];
+        if (tok0 >= n_new) return;
         n_tok = min(tt, n_new - tok0);
         first_pos = p.seq_pos0[seq] + tok0;
         const int skip = p.seq_skip[seq], end = first_pos + n_tok;
@@ -169,16 +169,15 @@ static int launch_prefix_merge(const PrefixParams& p, cudaStream_t stream) {
     return 0;
 }
 
-// The prefixes, the sequences' own keys, or both.
-static int launch_prefix_rows(const PrefixParams& p, bool prefixes, bool own, cudaStream_t stream) {
-    const int tt = kPrRows / p.group, own_tiles = (p.max_new + tt - 1) / tt;
-    const long prefix_tiles = prefixes ? prefix_tiles_bound(p, tt) : 0, tiles = prefix_tiles + (own ? (long)own_tiles * p.n_seqs : 0);
-    const int splits = prefixes && (!own || p.pieces > p.own_splits) ? p.pieces : p.own_splits;
+// The prefixes, or the sequences' own keys.
+static int launch_prefix_rows(const PrefixParams& p, bool own, cudaStream_t stream) {
+    const int tt = kPrRows / p.group, own_tiles = own ? (p.max_new + tt - 1) / tt : 0, splits = own ? p.own_splits : p.pieces;
+    const long tiles = own ? (long)own_tiles * p.n_seqs : prefix_tiles_bound(p, tt);
     MDMA_REQUIRE(tiles <= 0x7fffffffl && p.n_kv_heads <= 65535 && splits <= 65535, "prefix_attention: grid too large");
     auto run = [&](auto kernel, int dmax) -> int {
         const int bytes = 5 * kPrRows * dmax * 2;
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) e = launch_chained(kernel, dim3((unsigned)tiles, p.n_kv_heads, splits), dim3(kPrThreads), bytes, stream, p, (int)prefix_tiles, own_tiles);
+        if (e == cudaSuccess) e = launch_chained(kernel, dim3((unsigned)tiles, p.n_kv_heads, splits), dim3(kPrThreads), bytes, stream, p, own_tiles);
         if (e != cudaSuccess) return fail("prefix_attention: launch failed: %s", cudaGetErrorString(e));
         return 0;
     };
@@ -280,12 +279,12 @@ extern "C" int mdma_prefix_attention(const long long* words, int n_words, float 
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return fail("prefix_attention: no CUDA device");
     if (p.pieces > 0) {
-        if (int rc = kind == 0 ? launch_prefix_tc(p, stream) : kind == 1 ? launch_prefix_stream<true>(p, sms, stream) : launch_prefix_rows(p, true, false, stream)) return rc;
+        if (int rc = kind == 0 ? launch_prefix_tc(p, stream) : kind == 1 ? launch_prefix_stream<true>(p, sms, stream) : launch_prefix_rows(p, false, stream)) return rc;
         if (p.whole && p.pieces == 1) return 0;
     }
     if (!p.whole) {
         const bool stream_own = prefix_stream_fits(p);
-        if (int rc = stream_own ? launch_prefix_stream<false>(p, sms, stream) : launch_prefix_rows(p, false, true, stream)) return rc;
+        if (int rc = stream_own ? launch_prefix_stream<false>(p, sms, stream) : launch_prefix_rows(p, true, stream)) return rc;
         if (stream_own && p.own_splits == 1) return 0;
     }
     return launch_prefix_merge(p, stream);

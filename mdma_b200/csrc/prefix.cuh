@@ -179,7 +179,11 @@ static inline int prefix_params(const long long* w, int n_words, float scale, Pr
     MDMA_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0, "prefix_attention: %d heads over %d kv heads", p.n_heads, p.n_kv_heads);
     MDMA_REQUIRE(p.head_dim > 0 && p.head_dim <= 256, "prefix_attention: head_dim %d is beyond the limit of 256", p.head_dim);
     MDMA_REQUIRE(p.page_table && p.page_size > 0 && p.max_pages > 0, "prefix_attention: bad cache geometry");
-    MDMA_REQUIRE(p.n_groups >= 0 && p.n_shared >= 0 && p.n_shared <= p.n_groups && p.n_seqs >= 0 && p.n_tokens >= 0 && p.max_new >= 0 && p.pieces >= 0 && p.own_splits >= 0 && p.own_keys >= 0 && p.pieces + p.own_splits > 0, "prefix_attention: bad sizes");
+    MDMA_REQUIRE(p.n_groups >= 0 && p.n_shared >= 0 && p.n_shared <= p.n_groups && p.n_seqs >= 0 && p.n_tokens >= 0 &&
+                     (p.n_tokens == 0 || (p.max_new > 0 && p.n_groups > 0)),
+                 "prefix_attention: %d tokens of %d sequences in %d groups, %d with a prefix, at most %d of one", p.n_tokens, p.n_seqs,
+                 p.n_groups, p.n_shared, p.max_new);
+    MDMA_REQUIRE(p.pieces >= 0 && p.own_splits >= 0 && p.own_keys >= 0 && p.pieces + p.own_splits > 0, "prefix_attention: bad pieces");
     MDMA_REQUIRE(p.pieces <= 32 && p.own_splits <= 32, "prefix_attention: %d and %d pieces are beyond the limit of 32", p.pieces, p.own_splits);
     MDMA_REQUIRE(scale > 0.f, "prefix_attention: the score scale must be positive");
     p.group = p.n_heads / p.n_kv_heads;
