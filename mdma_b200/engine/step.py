@@ -17,6 +17,7 @@ less a reserve (src/model/planning.rs:55-125, src/bin/mdma/run.rs:66-71).
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from types import SimpleNamespace
 from typing import Optional, Sequence
 
 import numpy as np
@@ -91,6 +92,7 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
     `shares`: with room for steps that read shared prefixes once (without it forks read sequence by sequence)."""
     from ..sampling.sampler import DeviceSampler
     lay = Layout()
+    shares = shares and any(getattr(part, "prefix_shapes", list)() for part in model.all_parts())
     expected = model.expected_tensors()
 
     def held(name, ts):
@@ -140,8 +142,6 @@ def lay_out(model: DecoderModel, carver: Carver, *, dtype, device, sms: int, max
 def prefix_floats(model: DecoderModel, dtype, sms: int, max_slots: int, max_context: int, page_size: int) -> int:
     """Scratch for single-token steps over shared prefixes: the parts of every sequence's softmaxes, of 512 sequences at most
     (steps of more tokens use it as far as it goes; those that it does not hold read sequence by sequence)."""
-    from types import SimpleNamespace
-
     from .. import ops, ops_tensor
     ctx = SimpleNamespace(max_new=1, n_seqs=max_slots, n_tokens=max_slots, most_seqs=max_slots)
     most = SimpleNamespace(most_len=max_context, most_own=max_context, most_tokens=max_slots, n_groups=1, n_shared=1)
@@ -308,6 +308,9 @@ class Engine:
             tables = Carver(lay.tables)
             self.rt.alloc = tables.taker("tables")
             self.model.bind(lay.tensors, self.rt)
+            # parts that may read shared prefixes once, one of each kind
+            self._sharing = list({(type(part), tuple(part.prefix_shapes()), getattr(part, "_fast_ok", False)): part for part in self.model.all_parts()
+                                  if getattr(part, "prefix_shapes", list)()}.values())
             self.cache = lay.cache
             self.workspace = lay.workspace
             self.logits = lay.logits
@@ -428,7 +431,7 @@ class Engine:
         return slots <= self.max_slots and pages <= self.cache.n_pages
 
     def prefix_groups(self, slots: Sequence[int], pos0: Sequence[int], new: Sequence[int]):
-        """Who shares what in a step of these sequences, or None where nobody does.  Of single tokens the bounds are rounded to
+        """Who shares what in a step of these sequences, or None where nobody does or no layer would read it once.  Of single tokens the bounds are rounded to
         multiples of 1,024 as the replayed graphs see them (a graph serves every batch within its bounds), so that a step on
         its own adds up in the same order."""
         shared = [(length, members) for length, members in self.cache.shared_prefixes(slots)
@@ -436,6 +439,7 @@ class Engine:
         if not shared:
             return None
         groups = PrefixGroups(shared, pos0, new)
+        sizes = SimpleNamespace(max_new=max(new), n_seqs=len(new), n_tokens=sum(new), most_seqs=self.max_slots, most_len=self.max_context)
         if max(new) == 1:
             up = lambda n: min(self.max_context, -(-n // 1024) * 1024)  # noqa: E731
             groups.most_len, groups.most_own = up(groups.most_len), up(groups.most_own)
@@ -445,7 +449,7 @@ class Engine:
                 groups.shared_keys = 1 << max(10, (self.cache.shared_keys(those) - 1).bit_length())
             else:
                 groups.shared_keys = 0
-        return groups
+        return groups if any(part.shares(sizes, groups, self.page_size) for part in self._sharing) else None
 
     # ---- the step ----------------------------------------------------------
     def _validate(self, entries: Sequence[StepEntry]) -> None:

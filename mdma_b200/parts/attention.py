@@ -270,14 +270,17 @@ class Attention(Part):
 
     def _shares(self, ctx, view) -> bool:
         """Whether this step's attention reads shared prefixes once: sequences of the step have forked from one another, every key stays
-        in sight, and the parts fit the engine's scratch."""
-        g = getattr(ctx, "prefix", None)
-        if g is None or view.window or not self.prefix_shapes():
+        in sight, it pays, and the parts fit the engine's scratch."""
+        return getattr(ctx, "prefix", None) is not None and not view.window and self.shares(ctx, ctx.prefix, view.page_size)
+
+    def shares(self, ctx, g, page_size: int) -> bool:
+        """The same of the groups `g` and of `ctx`'s sizes alone."""
+        if not self.prefix_shapes():
             return False
         if self._fast_ok:
             from .. import ops_tensor
             pieces, own, _ = ops_tensor.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads, self.head_dim,
-                                                    self.rt.tc.sms if self.rt.tc is not None else 148, view.page_size)
+                                                    self.rt.tc.sms if self.rt.tc is not None else 148, page_size)
             if pieces == 0:              # every sequence by itself: so do the kernels of steps that share nothing
                 return False
             parts = pieces + own

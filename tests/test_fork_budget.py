@@ -43,3 +43,30 @@ def test_a_budget_without_room_for_shared_prefixes(cfg):
     assert np.abs(got[0] - got[1]).max() <= 2 * TOL_F32 * max(1.0, np.abs(got[0]).max())
     outs = [eng.generate([ids(cfg, 40, 7)], max_tokens=8, n=2)[1].tokens for eng in (whole, small)]
     assert outs[0] == outs[1] and len(outs[0]) == 8
+
+
+@pytest.mark.gpu
+def test_steps_that_gain_nothing_are_steps_without_groups():
+    """Forks of a short prompt in bfloat16 are read by every sequence: no tables go up, and the graphs of steps without forks
+    serve them."""
+    d, _, _ = make_model(TINY_D, 2, torch.bfloat16, std_scale=SHARP)
+    eng = engine(d, "bfloat16")
+    eng.generate([ids(TINY_D, 40, i) for i in range(4)], max_tokens=6)
+    session = eng.decode_session()
+    graphs = dict(session.graphs)
+    eng.generate([ids(TINY_D, 50, 9)], max_tokens=6, n=4)
+    eng.generate([ids(TINY_D, 60, 9)], max_tokens=6, n=2)
+    assert all(len(key) == 3 for key in session.graphs) and all(session.graphs[key] is g for key, g in graphs.items())
+
+
+@pytest.mark.gpu
+def test_layers_that_never_share_need_no_groups():
+    import gevonex_tiny
+    from mdma_b200.engine import Engine
+    d = gevonex_tiny.make_model(gevonex_tiny.CFG_A, 3)[0]
+    eng = Engine(d, dtype="float32", max_batch=4, max_context=96, page_size=16)
+    assert (not eng._sharing) == (not any(getattr(p, "prefix_shapes", list)() for p in eng.model.all_parts()))
+    a = eng.acquire()
+    step(eng, [(a, list(range(3, 40)), [0])])
+    slots = [a] + eng.fork(a, 2)
+    assert (eng.prefix_groups(slots, [37] * 3, [1] * 3) is None) == (not eng._sharing)
