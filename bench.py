@@ -4,6 +4,7 @@
     python bench.py [--gpus 1] [--steps K] [--warmup W] [--impl reference]
     python bench.py --shape llama-2-7b | llama-3.2-1b [--batch B] [--prompt-len P] [--prefill-tokens T]
     python bench.py --compare gevonex|mogevik|tubusun|fizadra|degavik|salipel [--compare-widths 1024,2048,4096] [--compare-layers 4]
+    python bench.py --completions N [--prompt-len P] [--layers L]
 
 Prints ONE JSON line.  The default run has the layer sizes of the
 Llama-3.1-8B shape with random bfloat16 weights, a batch of 8 sequences
@@ -46,6 +47,9 @@ heads are mixed) and a Llama.
 chunks, differential attention, a window that keeps the first tokens side by
 side with a matrix memory, dense and routed feed-forwards) beside a Tubusun
 (windowed attention side by side with linear attention) and a Llama.
+
+`--completions N`: N completions of one prompt (`Engine.generate(..., n=N)`, the prompt computed, kept and read once)
+beside the same prompt given N times, time to the first tokens and a step, through the Python entry point.
 """
 from __future__ import annotations
 
@@ -401,6 +405,38 @@ def compare(args) -> int:
     return 0
 
 
+def completions(args) -> int:
+    """N completions of a prompt beside N prompts: wall-clock time from a call to its tokens."""
+    import torch
+    from mdma_b200.engine import Engine
+    shape_name, cfg = SHAPES[args.shape]
+    layers = args.layers or cfg["num_hidden_layers"]
+    n, new = args.completions, 64
+    eng = Engine(config=dict(cfg, num_hidden_layers=layers), seed=0, dtype=args.dtype, max_batch=n,
+                 max_context=args.prompt_len + new + 1)
+    prompt = torch.randint(0, cfg["vocab_size"], (args.prompt_len,), generator=torch.Generator().manual_seed(0)).tolist()
+
+    def seconds(prompts, tokens, **kw):
+        times = []
+        for i in range(5):                       # the first two load kernels and capture graphs
+            torch.cuda.synchronize()
+            t = time.perf_counter()
+            outs = eng.generate(prompts, max_tokens=tokens, stop_ids=(), **kw)
+            times.append(time.perf_counter() - t)
+            assert len(outs) == n and all(len(o.tokens) == tokens for o in outs)
+        return sorted(times[2:])[1]
+
+    clock = ClockSampler()
+    clock.start()
+    row = {}
+    for name, prompts, kw in (("completions", [prompt], {"n": n}), ("prompts", [prompt] * n, {})):
+        first, whole = seconds(prompts, 1, **kw), seconds(prompts, 1 + new, **kw)
+        row[name] = {"first_ms": round(first * 1e3, 2), "ms_per_step": round((whole - first) * 1e3 / new, 3)}
+    print(json.dumps({"compare": f"{n} completions of one prompt beside {n} prompts", "model": shape_name, "layers": layers,
+                      "prompt_len": args.prompt_len, "steps": new, "dtype": args.dtype, **row, "clocks": clock.stop()}))
+    return 0
+
+
 def main() -> int:
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -424,8 +460,11 @@ def main() -> int:
                     help="another program: the named architecture beside a Llama of equal size (see the header)")
     ap.add_argument("--compare-widths", default="1024,2048,4096")
     ap.add_argument("--compare-layers", type=int, default=4)
+    ap.add_argument("--completions", type=int, default=None, metavar="N", help="N completions of one prompt beside N prompts")
     args = ap.parse_args()
 
+    if args.completions is not None and args.impl != "reference":
+        return completions(args)
     if args.compare is not None and args.impl != "reference":
         return compare(args)
     if args.impl == "reference":
