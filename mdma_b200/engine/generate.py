@@ -166,7 +166,9 @@ class Generator:
                 outputs[s.request].finish_reason = FINISH_CANCELLED
         try:
             if cancelled is not None and cancelled():
-                cancel_all()
+                for _, of in batch:
+                    for r in of:
+                        outputs[r].finish_reason = FINISH_CANCELLED
                 return
             # all prompts of the batch in one step
             entries = [StepEntry(s.slot, list(prompts[i]), [len(prompts[i]) - 1]) for s, (i, _) in zip(live, batch)]

@@ -91,3 +91,18 @@ def test_a_truncation_whose_copy_fails_changes_nothing(free, monkeypatch):
     for (group, src, dst, rows), g in zip(calls[1:], c.groups):
         assert group is g and src == [g.seq_pages[a][1]] and dst == [g.seq_pages[b][1]] and rows == [36] and src != dst
     assert len(calls) == 3 and c.length(b) == 100 and all(sorted(g.seq_pages[b]) == [0, 1] for g in c.groups)
+
+
+@pytest.mark.parametrize("after", [0, 1, 3])
+def test_cancelled_completions_say_so(after):
+    """Cancelled before the prompt, or after some tokens: every completion ends with that reason and no slot stays held."""
+    from mdma_b200.engine.generate import FINISH_CANCELLED, Generator
+    from test_forks import FakeEngine, FakeSampler
+    engine, asked = FakeEngine(8, 100), []
+
+    def cancelled():
+        asked.append(1)
+        return len(asked) > after
+    outs = Generator(engine, FakeSampler(), use_graphs=False).generate([[1, 2, 3], [4]], 9, n=3, cancelled=cancelled)
+    assert [o.finish_reason for o in outs] == [FINISH_CANCELLED] * 6 and not engine.live
+    assert all(len(o.tokens) == after for o in outs)
