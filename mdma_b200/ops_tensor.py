@@ -736,6 +736,22 @@ def prefix_plan(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, sms: int, 
     return pieces, own, PREFIX_ROWS
 
 
+def prefix_pays(ctx, g, n_heads: int, n_kv_heads: int, head_dim: int, page_size: int) -> bool:
+    """Whether a step that has a plan for its shared prefixes is faster with it than with every sequence reading by itself.
+    us of a call, by itself / shared, heads of 128.  Several tokens of up to 64 query rows a kv head (by itself on the mma.sync kernel),
+    32/8 heads: 2 tokens behind 64 16 / 21, 3 behind 512 23 / 29, behind 1,024 31 / 25, behind 4,096 68 / 29; 32/32: 20 behind 64 18 / 23,
+    30 behind 256 66 / 43.  More rows (by itself on tcgen05), 32/8: 8 x 500 behind 512 102 / 117, 24 x 60 behind 1,024 61 / 72, behind 1,536
+    82 / 86, behind 4,100 113 / 90; 2 x 1,000 behind 2,048 135 / 127; on pages of 16 tokens, where both are on mma.sync, 8 x 500 behind 2,048
+    1,485 / 1,569.  Single tokens on such pages: 2 behind 64 14 / 23, 4 behind 300 31 / 29."""
+    key = n_kv_heads * head_dim * 4                # bytes
+    if ctx.max_new == 1:
+        return (prefix_streams(ctx, n_heads // n_kv_heads, page_size) or g.most_len > PREFIX_SHORT
+                or g.shared_keys * key > min(PREFIX_LEAST_BYTES, 1024 * key))
+    if ctx.max_new * (n_heads // n_kv_heads) <= 64:
+        return g.most_len * key > PREFIX_LEAST_BYTES // 32
+    return page_size % 64 == 0 and (g.most_len > PREFIX_SHORT or g.shared_keys * key > PREFIX_LEAST_BYTES)
+
+
 def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                      sink_log2: Optional[torch.Tensor] = None, st: Optional[TensorState] = None) -> None:
     """`ops.prefix_attention` in bfloat16 on the tensor cores (the geometries of `attention_supported`).  `sink_log2`: the sinks

@@ -281,7 +281,8 @@ class Attention(Part):
             from .. import ops_tensor
             pieces, own, _ = ops_tensor.prefix_plan(ctx, g, self.n_heads, self.n_kv_heads, self.head_dim,
                                                     self.rt.tc.sms if self.rt.tc is not None else 148, page_size)
-            if pieces == 0:              # every sequence by itself: so do the kernels of steps that share nothing
+            # every sequence by itself: so do the kernels of steps that share nothing
+            if pieces == 0 or not ops_tensor.prefix_pays(ctx, g, self.n_heads, self.n_kv_heads, self.head_dim, page_size):
                 return False
             parts = pieces + own
             if parts == 1:

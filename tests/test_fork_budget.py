@@ -70,3 +70,44 @@ def test_layers_that_never_share_need_no_groups():
     step(eng, [(a, list(range(3, 40)), [0])])
     slots = [a] + eng.fork(a, 2)
     assert (eng.prefix_groups(slots, [37] * 3, [1] * 3) is None) == (not eng._sharing)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64])
+def test_small_prefixes_shared_by_force(monkeypatch, page):
+    """Whatever pays: prompts and single tokens through the kernels of shared prefixes, on pages of either kind."""
+    from mdma_b200 import ops_tensor
+    from test_forks import TINY_B, shared_whatever_the_size, test_forked_sequences_against_the_plain_implementation as forked
+    plans = shared_whatever_the_size(monkeypatch, 0)
+    kinds = set()
+    real = ops_tensor.prefix_attention
+    monkeypatch.setattr(ops_tensor, "prefix_attention", lambda ctx, *a, **k: (kinds.add(ctx.max_new > 1), real(ctx, *a, **k))[1])
+    forked("bfloat16", TINY_B, page)
+    assert kinds == {True, False} and plans
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cfg", [TINY_A, TINY_D], ids="AD")
+def test_prompts_behind_a_long_prefix(cfg, monkeypatch):
+    """Several tokens a sequence behind a prefix that pays by the rule itself, beside a prompt that shares nothing."""
+    from mdma_b200 import ops_tensor
+    from mdma_b200.engine import Engine
+    from plain_llama import plain_forward
+    from replay_util import assert_close
+    monkeypatch.setattr(ops_tensor, "PREFIX_SHORT", 60)
+    d, c, tensors = make_model(cfg, 1, torch.bfloat16, std_scale=SHARP)
+    weights = {k: v.float() for k, v in tensors.items()}
+    eng = Engine(d, dtype="bfloat16", max_batch=6, max_context=256, logit_rows=8)
+    used = []
+    real = ops_tensor.prefix_attention
+    monkeypatch.setattr(ops_tensor, "prefix_attention", lambda ctx, *a, **k: (used.append(ctx.max_new), real(ctx, *a, **k))[1])
+    text = ids(cfg, 70, 0)
+    a = eng.acquire()
+    step(eng, [(a, text)])
+    slots = [a] + eng.fork(a, 2)
+    lone = eng.acquire()
+    news = [ids(cfg, n, 5 + n) for n in (40, 1, 33, 50)]
+    got = step(eng, [(s, t, [len(t) - 1]) for s, t in zip(slots + [lone], news)])
+    want = [plain_forward(c, weights, (text if i < 3 else []) + t, torch.float64).numpy()[-1] for i, t in enumerate(news)]
+    assert_close(got, np.stack(want), "bfloat16", "prompts")
+    assert used == [50] * c.num_hidden_layers if hasattr(c, "num_hidden_layers") else set(used) == {50}

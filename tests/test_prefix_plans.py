@@ -48,3 +48,13 @@ def test_the_cache_remembers_what_families_shared():
     assert c.shared_keys([a, d] + new[1:]) == 2 * 128 + 4 * 70
     g = PrefixGroups([(70, [0, 2]), (128, [1])], [80, 200, 70, 9], [1] * 4)
     assert g.shared_keys == 2 * 70 + 128 and g.skips == [70, 128, 70, 0]
+
+
+@pytest.mark.parametrize("members, length, new, kv_heads, page, pays", [
+    (2, 64, 2, 8, 64, False), (4, 512, 3, 8, 64, False), (4, 1024, 3, 8, 64, True), (16, 256, 30, 32, 64, True), (2, 64, 20, 32, 64, False),
+    (8, 512, 500, 8, 64, False), (24, 1024, 60, 8, 64, False), (64, 1024, 60, 8, 64, True), (24, 4100, 60, 8, 64, True), (2, 2048, 1000, 8, 64, True),
+    (8, 2048, 500, 8, 16, False), (4, 2048, 3, 8, 16, True), (2, 64, 1, 8, 16, False), (4, 300, 1, 8, 16, True), (2, 4000, 1, 8, 16, True)])
+def test_steps_that_gain_nothing_read_by_themselves(members, length, new, kv_heads, page, pays):
+    g = PrefixGroups([(length, list(range(members)))], [length] * members, [new] * members)
+    ctx = SimpleNamespace(max_new=new, n_seqs=members, n_tokens=new * members, most_seqs=64, most_len=16384)
+    assert ops_tensor.prefix_pays(ctx, g, 32, kv_heads, 128, page) == pays
