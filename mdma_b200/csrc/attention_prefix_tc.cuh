@@ -18,8 +18,9 @@
 // row (the issue slots of sixteen softmax warps are the bound then) 4,200; a warp that issues for each tile, both in step, 4,850;
 // P V behind the whole softmax 3,450; steps of 64 keys with two places for S (products of N = 64 cost as much as of N = 128)
 // 3,700; the first half's weights before the row's maximum is known 3,450; a quarter of the exponentials by a polynomial on the
-// multiply-add units 3,400; the two tiles' exponentials in turns (a barrier for every pair of warps) 3,650; the next blocks asked into L2 ahead, 15% more where they come from memory.
-// 8,960 rows a kv head over 8,000 keys, 32 heads of 128: 320 us, 1.0 PFLOP/s.
+// multiply-add units 3,400; the two tiles' exponentials in turns (a barrier for every pair of warps) 3,650; the next blocks asked into
+// L2 ahead, 15% more where they come from memory.
+// 8,960 rows a kv head over 8,000 keys, 32 heads of 128: 307 us, 1.04 PFLOP/s; 337 to 351 and 0.91 in long runs, at the power limit.
 //
 // The list: the prefix's blocks, which all rows see, and (`whole`) behind them the own blocks of every sequence with tokens in the
 // tiles, which only that sequence's rows see: the others' lanes of O are left out of the product, so that what they are
@@ -261,7 +262,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) ptx::mma_bf16_ts(o, pa + i * 8, vd + ((i * 16 * 128) >> 4), idesc_o);
                             } else {
-                                const uint4 off = make_uint4(off_lanes(ra[t], rb[t], 0), off_lanes(ra[t], rb[t], 1), off_lanes(ra[t], rb[t], 2), off_lanes(ra[t], rb[t], 3));
+                                const uint4 off = make_uint4(off_lanes(ra[t], rb[t], 0), off_lanes(ra[t], rb[t], 1),
+                                                             off_lanes(ra[t], rb[t], 2), off_lanes(ra[t], rb[t], 3));
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) ptx::mma_bf16_ts(o, pa + i * 8, vd + ((i * 16 * 128) >> 4), idesc_o, off);
                             }
@@ -449,7 +451,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     ptx::tmem_load_wait();
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
-                        *reinterpret_cast<float4*>(stage + lane * kPtStage + c * 32 + q * 4) = make_float4(v[4 * q] * inv, v[4 * q + 1] * inv, v[4 * q + 2] * inv, v[4 * q + 3] * inv);
+                        *reinterpret_cast<float4*>(stage + lane * kPtStage + c * 32 + q * 4) =
+                            make_float4(v[4 * q] * inv, v[4 * q + 1] * inv, v[4 * q + 2] * inv, v[4 * q + 3] * inv);
                 }
             }
             __syncwarp();

@@ -309,8 +309,8 @@ class Engine:
             self.rt.alloc = tables.taker("tables")
             self.model.bind(lay.tensors, self.rt)
             # parts that may read shared prefixes once, one of each kind
-            self._sharing = list({(type(part), tuple(part.prefix_shapes()), getattr(part, "_fast_ok", False)): part for part in self.model.all_parts()
-                                  if getattr(part, "prefix_shapes", list)()}.values())
+            sharing = [part for part in self.model.all_parts() if getattr(part, "prefix_shapes", list)()]
+            self._sharing = list({(type(p), tuple(p.prefix_shapes()), getattr(p, "_fast_ok", False)): p for p in sharing}.values())
             self.cache = lay.cache
             self.workspace = lay.workspace
             self.logits = lay.logits
@@ -431,9 +431,9 @@ class Engine:
         return slots <= self.max_slots and pages <= self.cache.n_pages
 
     def prefix_groups(self, slots: Sequence[int], pos0: Sequence[int], new: Sequence[int]):
-        """Who shares what in a step of these sequences, or None where nobody does or no layer would read it once.  Of single tokens the bounds are rounded to
-        multiples of 1,024 as the replayed graphs see them (a graph serves every batch within its bounds), so that a step on
-        its own adds up in the same order."""
+        """Who shares what in a step of these sequences, or None where nobody does or no layer would read it once.  Of single
+        tokens the bounds are rounded to multiples of 1,024 as the replayed graphs see them (a graph serves every batch within its
+        bounds), so that a step on its own adds up in the same order."""
         shared = [(length, members) for length, members in self.cache.shared_prefixes(slots)
                   if all(pos0[m] >= length for m in members)] if self.reads_shared else []
         if not shared:

@@ -670,8 +670,9 @@ def prefix_streams(ctx, group: int, page_size: int) -> bool:
 def prefix_own_cut(ctx, most_own: int, n_kv_heads: int, sms: int) -> tuple[int, int]:
     """(pieces, keys of a piece) of the own keys of single tokens that are streamed: one block a (sequence, kv head) joins
     everything itself up to a piece's keys.  Keys beyond are cut into pieces of a fixed length, so that a step does not wait for the
-    one long sequence's blocks; their length follows from the most sequences and the longest context that the engine can hold.  Only their number follows from the live ones: a sequence's keys are cut at the same places, and its parts
-    joined in the same order, whoever shares the step."""
+    one long sequence's blocks; their length follows from the most sequences and the longest context that the engine can hold.
+    Only their number follows from the live ones: a sequence's keys are cut at the same places, and its parts joined in the same
+    order, whoever shares the step."""
     return _own_cut(getattr(ctx, "most_seqs", None) or ctx.n_seqs, max(most_own, getattr(ctx, "most_len", None) or 0), most_own, n_kv_heads, sms,
                     PREFIX_OWN_KEYS // 4)
 
