@@ -87,14 +87,16 @@ attention_finish_kernel(const FinishParams p, const TO* __restrict__ gate, TO* _
         const float* ml = p.part_ml + row * p.splits * 2;
         float m = -INFINITY, l = 0.f;
         for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[2 * s]);
-        for (int s = 0; s < p.splits; ++s) if (ml[2 * s] != -INFINITY) l += exp2f(ml[2 * s] - m) * ml[2 * s + 1];
+        // (without a visible key: no maximum and no sum; a maximum passes over NaN, the sum does not)
+        auto seen = [&](int s) { return ml[2 * s] != -INFINITY || ml[2 * s + 1] != 0.f; };
+        for (int s = 0; s < p.splits; ++s) if (seen(s)) l += exp2f(ml[2 * s] - m) * ml[2 * s + 1];
         if (p.sink_log2) l += exp2f(p.sink_log2[h] - m);
         const float share = f / l;
         float a[4 * NQ];
 #pragma unroll
         for (int i = 0; i < 4 * NQ; ++i) a[i] = 0.f;
         for (int s = 0; s < p.splits; ++s) {
-            if (ml[2 * s] == -INFINITY) continue;                       // a run without a visible key
+            if (!seen(s)) continue;                                     // a run without a visible key
             const float w = exp2f(ml[2 * s] - m);
             const float* src = p.part_o + (row * p.splits + s) * p.v_dim;
             quads([&](int d, int i, int n) {

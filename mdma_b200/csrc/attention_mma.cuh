@@ -30,6 +30,10 @@ constexpr int kRows = 64;        // query rows per block (4 warps x 16)
 constexpr int kKeys = 64;        // keys per block of the stream
 constexpr int kAttnThreads = 128;
 
+// Whether a part of a softmax has seen a key: one that has not leaves no maximum and no sum.  (The maximum passes over NaN: a part
+// whose scores are all NaN leaves no maximum either, but a sum that is NaN.)
+__device__ __forceinline__ bool attn_has_keys(float m, float l) { return m != -INFINITY || l != 0.f; }
+
 struct AttnParams {
     const __nv_bfloat16* q; int q_stride;          // rows of the fused projection; queries first
     const __nv_bfloat16* k_cache; const __nv_bfloat16* v_cache;   // [pages, page_size, kv_heads, head_dim]
@@ -464,10 +468,10 @@ attention_decode_kernel(const AttnParams p) {
         float l = 0.f, acc = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float mw = comb[((size_t)w * 16 + r) * kRowF + DMAX];
-            if (mw != -INFINITY) {
+            const float mw = comb[((size_t)w * 16 + r) * kRowF + DMAX], lw = comb[((size_t)w * 16 + r) * kRowF + DMAX + 1];
+            if (attn_has_keys(mw, lw)) {
                 const float f = exp2f(mw - m);
-                l += f * comb[((size_t)w * 16 + r) * kRowF + DMAX + 1];
+                l += f * lw;
                 acc += f * comb[((size_t)w * 16 + r) * kRowF + d];
             }
         }
@@ -803,9 +807,9 @@ attention_decode_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         for (int w = 0; w < NW; ++w) m = fmaxf(m, top[w * 16 + r]);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float mw = top[w * 16 + r];
+            const float mw = top[w * 16 + r], lw = top[(NW + w) * 16 + r];
             float f = -1.f;                                 // a warp without keys has no share
-            if (mw != -INFINITY) { f = exp2f(mw - m); l += f * top[(NW + w) * 16 + r]; }
+            if (attn_has_keys(mw, lw)) { f = exp2f(mw - m); l += f * lw; }
             top[(2 * NW + w) * 16 + r] = f;
         }
         top[r] = m; top[NW * 16 + r] = l;
@@ -861,12 +865,12 @@ __global__ void attention_merge_kernel(const float* __restrict__ part_o, const f
     float m = -INFINITY;
     for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[s * 2]);
     float l = 0.f;
-    for (int s = 0; s < splits; ++s) if (ml[s * 2] != -INFINITY) l += exp2f(ml[s * 2] - m) * ml[s * 2 + 1];
+    for (int s = 0; s < splits; ++s) if (attn_has_keys(ml[s * 2], ml[s * 2 + 1])) l += exp2f(ml[s * 2] - m) * ml[s * 2 + 1];
     if (sink_log2) l += exp2f(sink_log2[th % n_heads] - m);          // the sink counts once, whatever the split
     for (int d = threadIdx.x; d < head_dim; d += blockDim.x) {
         float acc = 0.f;
         for (int s = 0; s < splits; ++s)
-            if (ml[s * 2] != -INFINITY) acc += exp2f(ml[s * 2] - m) * part_o[(th * splits + s) * head_dim + d];
+            if (attn_has_keys(ml[s * 2], ml[s * 2 + 1])) acc += exp2f(ml[s * 2] - m) * part_o[(th * splits + s) * head_dim + d];
         out[th * head_dim + d] = __float2bfloat16_rn(acc / l);      // (as the kernel itself ends where nothing is split)
     }
 }
