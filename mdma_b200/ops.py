@@ -1239,18 +1239,17 @@ def prefix_checks(ctx, q, view, out, n_heads: int, n_kv_heads: int, head_dim: in
               g.seq_skip):
         if t.dtype is not int32 or t.get_device() != device or not t.is_contiguous():
             raise KernelError("positions, page tables and groups are contiguous int32, on the queries' device")
-    table = view.page_table.shape
-    if len(table) != 2 or table[1] != view.max_pages:
-        raise KernelError(f"a page table of {tuple(table)} does not hold {view.max_pages} pages a slot")
-    dtype, rows, shape = q.dtype, q.shape, out.shape
+    if view.page_table.dim() != 2 or view.page_table.size(1) != view.max_pages:
+        raise KernelError(f"a page table of {tuple(view.page_table.shape)} does not hold {view.max_pages} pages a slot")
+    dtype, rows, shape, cache = q.dtype, q.shape, out.shape, k.shape
     if (k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or len(rows) != 2 or q.stride(1) != 1
             or not (k.is_contiguous() and v.is_contiguous() and out.is_contiguous())):
         raise KernelError("queries, caches and results have one dtype; caches and results are contiguous")
-    if (n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads or len(k.shape) != 4 or k.shape != v.shape
-            or k.size(1) != view.page_size or k.size(2) != n_kv_heads or k.size(3) != head_dim or len(shape) != 2
+    if (n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads or len(cache) != 4 or cache != v.shape
+            or cache[1] != view.page_size or cache[2] != n_kv_heads or cache[3] != head_dim or len(shape) != 2
             or rows[0] < ctx.n_tokens or rows[1] < n_heads * head_dim or shape[0] < ctx.n_tokens or shape[1] != n_heads * head_dim):
         raise KernelError(f"{n_heads} heads over {n_kv_heads} kv heads of {head_dim} do not fit queries {tuple(q.shape)}, caches "
-                          f"{tuple(k.shape)} and results {tuple(out.shape)}")
+                          f"{tuple(cache)} and results {tuple(out.shape)}")
     if (g.group_len.numel() < g.n_groups or g.group_seq.numel() < g.n_groups or g.tok_first.numel() <= g.n_groups
             or g.toks.numel() < ctx.n_tokens or g.seq_skip.numel() < ctx.n_seqs or ctx.seq_start.numel() <= ctx.n_seqs
             or ctx.seq_pos0.numel() < ctx.n_seqs or ctx.seq_slot.numel() < ctx.n_seqs or ctx.tok_seq.numel() < ctx.n_tokens):

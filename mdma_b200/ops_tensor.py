@@ -769,7 +769,7 @@ def prefix_attention(ctx, q: torch.Tensor, view, out: torch.Tensor, n_heads: int
     flush_pending(q.device, st)
     g = ctx.prefix
     pieces, own, kind = prefix_plan(ctx, g, n_heads, n_kv_heads, head_dim, st.sms, view.page_size)
-    own_keys = prefix_own_cut(ctx, g.most_own, n_kv_heads, st.sms)[1] if pieces and own and ctx.max_new == 1 else 0
+    own_keys = prefix_own_cut(ctx, g.most_own, n_kv_heads, st.sms)[1] if pieces and own > 1 and ctx.max_new == 1 else 0
     need = ops.prefix_scratch_floats(ctx.n_tokens, n_heads, pieces + own, head_dim) if pieces + own > 1 else 0
     if own_st is not None:
         st.need(need, "attention over shared prefixes")
