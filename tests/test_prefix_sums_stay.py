@@ -116,3 +116,40 @@ def test_pieces_of_a_fixed_length(kind, monkeypatch):
     assert torch.equal(outs[0], outs[1])
     short = [i for i in range(ctx.n_seqs) if int(ctx.seq_pos0[i]) + 1 - int(ctx.prefix.seq_skip[i]) <= 128]
     assert len(short) == 4 and torch.equal(outs[0][short], outs[2][short])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", ["float32", "tcgen05", "streamed"])
+def test_runs_across_a_piece_of_own_keys(path, monkeypatch):
+    """Replayed runs in which the longest own keys pass 1,024 and a piece's end, bit for bit the steps on their own."""
+    from mdma_b200.engine import Engine
+    if path != "float32":
+        shared_whatever_the_size(monkeypatch, 0 if path == "tcgen05" else 1 << 20)
+        monkeypatch.setattr(ops_tensor, "PREFIX_OWN_KEYS", 2048)
+    d, _, _ = make_model(TINY_D, 2, torch.bfloat16, std_scale=SHARP)
+    out = []
+    for replayed in (True, False):
+        eng = Engine(d, dtype="float32" if path == "float32" else "bfloat16", max_batch=6, max_context=2304)
+        a = eng.acquire()
+        step(eng, [(a, ids(TINY_D, 70, 0))])
+        slots = [a] + eng.fork(a, 2)
+        step(eng, [(a, ids(TINY_D, 1020, 1)), (slots[1], ids(TINY_D, 40, 2))])
+        tokens, logits, chosen = [3, 4, 5], {}, []
+        if replayed:
+            session = eng.decode_session()
+            session.start(slots, tokens)
+            while len(chosen) < 12:
+                session.run(5)
+                chosen += [t for t, _ in session.read()]
+                logits[len(chosen)] = session.logits[:3].clone()
+        else:
+            for i in range(12):
+                rows = eng.step([(s, [t], [0]) for s, t in zip(slots, tokens)])
+                logits[i + 1] = rows.clone()
+                tokens = eng.sampler.sample(rows, eng.decode_session().params, [0, 1, 2], [0] * 3)[0]
+                chosen.append(tokens)
+        eng.check_status()
+        out.append((logits, chosen[:12]))
+    (replays, picked), (steps, alone) = out
+    assert picked == alone and any(n <= 4 for n in replays)          # (a run ended where the own keys reached 1,024)
+    assert all(torch.equal(rows, steps[n]) for n, rows in replays.items() if n in steps)
